@@ -67,6 +67,22 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+class _NoSwitch:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_SWITCH = _NoSwitch()
+
+
+def device_guard(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one, so that a launch and ``stream_ptr`` go to it."""
+    return _NO_SWITCH if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -75,7 +91,8 @@ _ERR = {1: "unsupported shape or alignment", 2: "CUDA runtime error", 3: "tensor
 
 
 LAUNCH_COUNT = 0  # kernel-launching library calls made by this process (a call may launch several kernels)
-_LAUNCHES_PER_CALL = {"sb_attn_bwd_varlen": 3, "sb_attn_decode_paged": 1}
+_LAUNCHES_PER_CALL = {"sb_attn_bwd_varlen": 3, "sb_attn_decode_paged": 1, "sb_qk_norm_rope_bwd": 2,
+                      "sb_moe_few_experts": 2}
 
 
 def check(code: int, what: str) -> None:

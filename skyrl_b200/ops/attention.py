@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -27,6 +28,7 @@ def _k():
         vp, ci, cf, cl = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
         lib.sb_attn_fwd_varlen.argtypes = [vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, cl, cf, vp]
         lib.sb_attn_bwd_varlen.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, cl, cf, vp]
+        lib.sb_paged_layout.argtypes = [vp, cl, ci, vp, vp, ci, ci, ci, vp, vp, vp, vp, vp]
         lib.sb_kv_cache_write.argtypes = [vp, vp, vp, vp, ci, ci, ci, ci, cl, ci, vp]
         lib.sb_attn_decode_paged.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, cl, cf, vp]
         lib.sb_attn_decode_paged_tc.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, cl, cf, vp]
@@ -184,6 +186,59 @@ def kv_cache_write(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ok = slots >= 0
     kc[slots[ok].long()] = k[ok]
     vc[slots[ok].long()] = v[ok]
+
+
+class PagedLayout(NamedTuple):
+    """Rows of a packed prefill batch (``paged_layout``); all int32."""
+
+    cu_seqlens: torch.Tensor  # [B + 1] first row of every sequence
+    positions: torch.Tensor   # [total] position of the row's token in its sequence (0 behind the last sequence)
+    slots: torch.Tensor       # [total] cache slot of the token, -1 where it has none
+    rows: torch.Tensor        # [total] the token's row in the layout of the whole sequences, -1 behind the last one
+
+
+def paged_layout(block_tables: torch.Tensor, lens: torch.Tensor, block_size: int, total: int,
+                 starts: torch.Tensor | None = None) -> PagedLayout:
+    """Offsets, positions and cache slots of the packed rows of ``B`` sequences, built on the device in one launch.
+
+    Sequence ``b`` has the tokens ``starts[b] .. lens[b] - 1`` (``starts``: tokens that are cached already; none when
+    omitted), one row each.  ``block_tables`` ``[B, max_blocks]``, ``lens`` and ``starts`` ``[B]`` are int32 and stay on
+    the device; ``total`` is the number of rows to lay out, which the caller knows from the lengths it scheduled or
+    bounds from above: rows behind the last sequence are padding, rows beyond ``total`` are left out.  A token behind
+    the table's last block, or in a block that the table marks with a negative entry, has slot -1."""
+    what = "paged_layout"
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError(f"{what}: block tables must be int32 [B, max_blocks] rows, got {block_tables.dtype} {tuple(block_tables.shape)}")
+    B = block_tables.shape[0]
+    for t in (lens, starts):
+        if t is not None and (t.shape != (B,) or t.dtype != torch.int32 or not t.is_contiguous() or t.device != block_tables.device):
+            raise ValueError(f"{what}: lengths must be contiguous int32 [{B}] tensors on the tables' device")
+    if not 0 <= total < 2**31 or block_size < 1:
+        raise ValueError(f"{what}: total {total} or block size {block_size} is out of range")
+    dev = block_tables.device
+    if dev.type == "cuda":
+        buf = torch.empty(B + 1 + 3 * total, device=dev, dtype=torch.int32)
+        lay = PagedLayout(*buf.split((B + 1, total, total, total)))
+        with _lib.device_guard(buf):
+            code = _k().sb_paged_layout(block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], _lib.ptr(starts),
+                                        lens.data_ptr(), B, block_size, total, *[t.data_ptr() for t in lay], _lib.stream_ptr())
+        _lib.check(code, "sb_paged_layout")
+        return lay
+    n = lens.long().clamp_min(0)
+    s = torch.zeros_like(n) if starts is None else torch.minimum(starts.long().clamp_min(0), n)
+    zero = n.new_zeros(1)
+    cu, whole = torch.cat([zero, (n - s).cumsum(0)]), torch.cat([zero, n.cumsum(0)])
+    seq = torch.repeat_interleave(torch.arange(B), n - s)[:total]
+    pos = torch.arange(seq.numel()) - cu[seq] + s[seq]
+    blk = pos // block_size
+    entry = torch.full_like(pos, -1)
+    inside = blk < block_tables.shape[1]
+    entry[inside] = block_tables[seq[inside], blk[inside]].long()
+    slot = torch.where(entry >= 0, entry * block_size + pos % block_size, torch.full_like(pos, -1))
+    out = [torch.full((total,), f, dtype=torch.int32) for f in (0, -1, -1)]
+    for o, v in zip(out, (pos, torch.where(slot < 2**31, slot, torch.full_like(slot, -1)), whole[seq] + pos)):
+        o[: v.numel()] = v.to(torch.int32)
+    return PagedLayout(cu.to(torch.int32), *out)
 
 
 def attn_decode_paged_ref(q, k_cache, v_cache, block_tables, ctx_lens, scale, sinks=None):

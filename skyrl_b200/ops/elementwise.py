@@ -10,6 +10,7 @@ device-kernel inventory).
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -114,11 +115,64 @@ def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------------------- RoPE
-def build_rope_table(max_pos: int, head_dim: int, theta: float, device) -> torch.Tensor:
-    """[max_pos, head_dim] fp32: cos in the first half of each row, sin in the second."""
-    inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim))
+def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
+    """``(inverse frequencies [rotary_dim / 2] in fp64, factor on cos and sin)`` of a rotary embedding.
+
+    ``scaling`` is the ``rope_scaling`` entry of a checkpoint's configuration; ``rope_type`` (or ``type``) is one of
+
+    * ``default``: no scaling;
+    * ``linear``: positions divided by ``factor``;
+    * ``llama3``: wavelengths above ``original_max_position_embeddings / low_freq_factor`` are divided by ``factor``,
+      those below ``original / high_freq_factor`` stay, and a linear ramp over the number of turns joins the two;
+    * ``yarn``: the pairs that turn fewer than ``beta_slow`` times over the original context are divided by ``factor``,
+      those above ``beta_fast`` stay, with a ramp over the pair index between; cos and sin are multiplied by
+      ``attention_factor`` (default ``0.1 ln(factor) + 1``)."""
+    inv = 1.0 / (theta ** (torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim))
+    kind = (scaling or {}).get("rope_type") or (scaling or {}).get("type") or "default"
+    if kind == "default":
+        return inv, 1.0
+    if kind not in ("linear", "llama3", "yarn"):
+        raise ValueError(f"rope scaling '{kind}' is not supported (default, linear, llama3, yarn)")
+    factor = float(scaling["factor"])
+    if not factor >= 1.0:
+        raise ValueError(f"rope scaling factor must be at least 1, got {factor}")
+    if kind == "linear":
+        return inv / factor, 1.0
+    orig = float(scaling["original_max_position_embeddings"])
+    if kind == "llama3":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not high > low:
+            raise ValueError("llama3 rope scaling needs high_freq_factor > low_freq_factor")
+        keep = ((orig * inv / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        return keep * inv + (1.0 - keep) * inv / factor, 1.0
+    fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
+
+    def pair_turning(n: float) -> float:  # index of the pair that turns n times over the original context
+        return rotary_dim * math.log(orig / (n * 2 * math.pi)) / (2 * math.log(theta))
+
+    lo, hi = pair_turning(fast), pair_turning(slow)
+    if scaling.get("truncate", True):
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
+    stretch = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+    gain = scaling.get("attention_factor")
+    if gain is None:
+        def mscale(m: float) -> float:
+            return 0.1 * m * math.log(factor) + 1.0
+
+        m, m_all = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        gain = mscale(float(m)) / mscale(float(m_all)) if m and m_all else mscale(1.0)
+    return stretch * inv / factor + (1.0 - stretch) * inv, float(gain)
+
+
+def build_rope_table(max_pos: int, head_dim: int, theta: float, device, scaling: dict | None = None) -> torch.Tensor:
+    """[max_pos, head_dim] fp32: cos in the first half of each row, sin in the second.  For heads that are rotated in
+    part, ``head_dim`` is the rotated width.  ``scaling``: see ``rope_frequencies``.  Angles are formed in fp64: at
+    position 131072 an fp32 angle would already be off by 2^-8."""
+    inv, gain = rope_frequencies(head_dim, theta, scaling)
     ang = torch.arange(max_pos, dtype=torch.float64)[:, None] * inv[None, :]
-    return torch.cat([ang.cos(), ang.sin()], dim=-1).float().to(device)
+    tab = torch.cat([ang.cos(), ang.sin()], dim=-1)
+    return (tab if gain == 1.0 else tab * gain).float().to(device)
 
 
 def _rope_ref(qkv, pos, table, n_rot_heads, D, sign):

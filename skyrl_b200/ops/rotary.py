@@ -1,0 +1,295 @@
+"""Rotary positions in their layouts, norms of query and key heads with the rotation in the same pass, and the serving
+form that also writes keys and values to the paged cache (``csrc/qk_rope.cu``).
+
+All three work on packed projection rows ``[T, heads * head_dim]`` (queries, then keys, then values) with int32 positions
+``[T]`` and the cos | sin table of ``elementwise.build_rope_table``.  The table's width is the rotated part of a head:
+elements behind it pass unchanged.  ``interleaved`` pairs neighbours ``(2i, 2i + 1)``; otherwise pairs are
+``(i, i + R / 2)``.  bf16, fp16 and fp32 rows; statistics and sums in fp32, one rounding per result.  A position outside
+the table gives NaN in the rotated elements.
+
+CUDA tensors run the kernels; CPU tensors run the PyTorch formulation below.  Reference behaviour: the attention modules
+that the reference runs under FSDP (skyrl/backends/skyrl_train/workers/model_wrapper.py:329-333).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_MAX_HEAD_DIM = 512
+_cfg_done = False
+
+
+def _k():
+    global _cfg_done
+    lib = _lib.kernels()
+    if not _cfg_done:
+        vp, ci, cf, cl = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
+        lib.sb_qk_rope_fwd.argtypes = [vp] * 9 + [cl] * 4 + [ci] * 10 + [cf, cf, vp]
+        lib.sb_qk_norm_rope_bwd_parts.argtypes = [ci, ci, ci]
+        lib.sb_qk_norm_rope_bwd.argtypes = [vp] * 10 + [ci] + [cl] * 3 + [ci] * 10 + [cf, vp]
+        _cfg_done = True
+    return lib
+
+
+# ----------------------------------------------------------------------------- checks
+def _check(rows, pos, table, nq, nk, head_dim, q_norm, k_norm, what):
+    T, W = rows.shape[-2], rows.shape[-1]
+    if nq < 0 or nk < 0 or nq + nk < 1 or head_dim < 1 or W % head_dim or W // head_dim < nq + nk:
+        raise ValueError(f"{what}: rows of width {W} do not hold {nq} + {nk} rotated heads of size {head_dim}")
+    if head_dim > _MAX_HEAD_DIM:
+        raise ValueError(f"{what}: head size {head_dim} is above {_MAX_HEAD_DIM}")
+    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        raise ValueError(f"{what}: the rope table must be a contiguous fp32 [positions, rotated width] tensor")
+    R = table.shape[1]
+    if R < 2 or R % 2 or R > head_dim or table.shape[0] < 1:
+        raise ValueError(f"{what}: rope table {tuple(table.shape)} does not fit heads of size {head_dim}")
+    if pos.dtype != torch.int32 or pos.dim() != 1 or pos.shape[0] != T or not pos.is_contiguous():
+        raise ValueError(f"{what}: positions must be a contiguous int32 [{T}] tensor, got {pos.dtype} {tuple(pos.shape)}")
+    if (q_norm is None) != (k_norm is None):
+        raise ValueError(f"{what}: q_norm and k_norm go together")
+    dev = rows.device
+    if pos.device != dev or table.device != dev:
+        raise ValueError(f"{what}: rows, positions and table must be on one device")
+    if q_norm is not None:
+        for w in (q_norm, k_norm):
+            if w.shape != (head_dim,) or not w.is_contiguous() or w.device != dev:
+                raise ValueError(f"{what}: norm weights must be contiguous [{head_dim}] tensors on the rows' device")
+
+
+def _check_rows(x, what):
+    if x.dim() != 2:
+        raise ValueError(f"{what}: rows must be [T, heads * head_dim], got {tuple(x.shape)}")
+    if x.dtype not in _DTYPE:
+        raise ValueError(f"{what}: rows must be bf16, fp16 or fp32, got {x.dtype}")
+
+
+def _row_major(x: torch.Tensor) -> torch.Tensor:
+    """Rows that the kernels can walk: unit stride inside a row, no two rows on the same memory."""
+    W = x.shape[1]
+    return x if (x.stride(1) == 1 or W == 1) and (x.stride(0) >= W or x.shape[0] <= 1) else x.contiguous()
+
+
+# ----------------------------------------------------------------------------- PyTorch formulation
+def _angles_ref(pos, table):
+    known = (pos >= 0) & (pos < table.shape[0])
+    cs = table[torch.where(known, pos, torch.zeros_like(pos)).long()]
+    cs = torch.where(known[:, None], cs, torch.full_like(cs, float("nan")))
+    return cs[:, None, : table.shape[1] // 2], cs[:, None, table.shape[1] // 2 :]
+
+
+def _rotate_ref(x, cos, sin, interleaved):
+    """``x``: fp32 ``[T, heads, D]``."""
+    R = 2 * cos.shape[-1]
+    if interleaved:
+        a, b = x[..., 0:R:2], x[..., 1:R:2]
+        rot = torch.stack([a * cos - b * sin, b * cos + a * sin], dim=-1).flatten(-2)
+    else:
+        a, b = x[..., : R // 2], x[..., R // 2 : R]
+        rot = torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+    return torch.cat([rot, x[..., R:]], dim=-1)
+
+
+def _fwd_ref(x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, sign):
+    T = x.shape[0]
+    cos, sin = _angles_ref(pos, table)
+    h = x.reshape(T, x.shape[1] // D, D)
+    parts = []
+    for lo, hi, w in ((0, nq, q_norm), (nq, nq + nk, k_norm)):
+        p = h[:, lo:hi].float()
+        if w is not None:
+            p = p * torch.rsqrt(p.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+        parts.append(_rotate_ref(p, cos, sin * sign, interleaved).to(x.dtype))
+    return torch.cat([*parts, h[:, nq + nk :]], dim=1).flatten(1)
+
+
+def _bwd_ref(dy, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved):
+    T = x.shape[0]
+    cos, sin = _angles_ref(pos, table)
+    d, h = dy.reshape(T, x.shape[1] // D, D), x.reshape(T, x.shape[1] // D, D)
+    dx, dws = [], []
+    for lo, hi, w in ((0, nq, q_norm), (nq, nq + nk, k_norm)):
+        g, p = _rotate_ref(d[:, lo:hi].float(), cos, -sin, interleaved), h[:, lo:hi].float()
+        r = torch.rsqrt(p.pow(2).mean(-1, keepdim=True) + eps)
+        xh = p * r
+        dws.append((g * xh).sum((0, 1)))
+        g = g * w.float()
+        dx.append((r * (g - xh * (g * xh).mean(-1, keepdim=True))).to(x.dtype))
+    return torch.cat([*dx, d[:, nq + nk :]], dim=1).flatten(1), dws[0], dws[1]
+
+
+# ----------------------------------------------------------------------------- kernels
+def _launch_fwd(src, dst, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, sign, n_part=0, slots=None,
+                k_cache=None, v_cache=None):
+    T, W = dst.shape
+    if T == 0:
+        return dst
+    with _lib.device_guard(dst):
+        code = _k().sb_qk_rope_fwd(
+            src.data_ptr(), dst.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), pos.data_ptr(), table.data_ptr(),
+            _lib.ptr(slots), _lib.ptr(k_cache), _lib.ptr(v_cache),
+            0 if k_cache is None else k_cache.shape[0] * k_cache.shape[1], src.stride(-2), dst.stride(0),
+            src.stride(0) if n_part else 0, n_part, table.shape[0], T, nq, nk, W // D, D, table.shape[1],
+            _DTYPE[dst.dtype], int(interleaved), eps, sign, _lib.stream_ptr())
+    _lib.check(code, "sb_qk_rope_fwd")
+    return dst
+
+
+class _QKNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved):
+        ctx.meta = (nq, nk, D, eps, interleaved)
+        if x.is_cuda:
+            x = _row_major(x)
+            out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+            _launch_fwd(x, out, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, 1.0)
+        else:
+            out = _fwd_ref(x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, 1.0)
+        if q_norm is None:
+            ctx.save_for_backward(pos, table)
+        else:
+            ctx.save_for_backward(pos, table, x, q_norm, k_norm)
+            # taken here, not from the saved tensors: activation checkpointing hands backward detached aliases
+            ctx.main_grads = (getattr(q_norm, "main_grad", None), getattr(k_norm, "main_grad", None))
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        nq, nk, D, eps, interleaved = ctx.meta
+        none = (None,) * 7
+        pos, table, *rest = ctx.saved_tensors
+        if not rest:
+            if not dy.is_cuda:
+                return _fwd_ref(dy, None, None, pos, table, nq, nk, D, eps, interleaved, -1.0), None, None, *none
+            dy = _row_major(dy)
+            dx = torch.empty(dy.shape, device=dy.device, dtype=dy.dtype)
+            return _launch_fwd(dy, dx, None, None, pos, table, nq, nk, D, eps, interleaved, -1.0), None, None, *none
+        x, q_norm, k_norm = rest
+        want = ctx.needs_input_grad[1:3]
+        if not dy.is_cuda:
+            dx, *dws = _bwd_ref(dy, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved)
+        else:
+            dx, *dws = _launch_bwd(dy, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, want, ctx.main_grads)
+        out = []
+        for dw, w, mg, on in zip(dws, (q_norm, k_norm), ctx.main_grads, want):
+            if not on or dw is None:
+                out.append(None)
+            elif mg is not None:
+                mg.add_(dw)
+                out.append(None)
+            else:
+                out.append(dw.to(w.dtype))
+        return dx, *out, *none
+
+
+def _launch_bwd(dy, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, want, main_grads):
+    """Returns ``(dx, dqw, dkw)``; a weight gradient that the kernel added to its fp32 ``main_grad`` is None."""
+    dy = _row_major(dy)
+    T, W = x.shape
+    dx = torch.empty((T, W), device=x.device, dtype=x.dtype)
+    wanted = [(g, w) for g, w, on in zip(main_grads, (q_norm, k_norm), want) if on]
+    # added in place where every wanted gradient has its fp32 buffer, stored in the weights' type where none has; a mix
+    # goes through fp32 zeros
+    direct = bool(wanted) and all(g is not None and g.is_contiguous() and g.dtype == torch.float32 for g, _ in wanted)
+    mixed = not direct and any(g is not None for g, _ in wanted)
+    dws = [None if not on else g if direct else torch.zeros_like(w, dtype=torch.float32) if mixed else torch.empty_like(w)
+           for g, w, on in zip(main_grads, (q_norm, k_norm), want)]
+    if T == 0:
+        return (dx, *(None if direct or g is None else g.zero_() for g in dws))
+    lib = _k()
+    n_parts = lib.sb_qk_norm_rope_bwd_parts(T, W // D, D)
+    part = torch.empty(n_parts * 2 * D, device=x.device, dtype=torch.float32) if wanted else None
+    with _lib.device_guard(x):
+        code = lib.sb_qk_norm_rope_bwd(
+            dy.data_ptr(), x.data_ptr(), dx.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), pos.data_ptr(),
+            table.data_ptr(), _lib.ptr(dws[0]), _lib.ptr(dws[1]), _lib.ptr(part), n_parts, dy.stride(0), x.stride(0),
+            dx.stride(0), table.shape[0], T, nq, nk, W // D, D, table.shape[1], _DTYPE[x.dtype], int(interleaved),
+            int(direct or mixed), eps, _lib.stream_ptr())
+    _lib.check(code, "sb_qk_norm_rope_bwd")
+    return (dx, None, None) if direct else (dx, *dws)
+
+
+# ----------------------------------------------------------------------------- entry points
+def rotary(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, n_rot_heads: int, head_dim: int,
+           interleaved: bool = False) -> torch.Tensor:
+    """Rotate the first ``n_rot_heads`` heads of every row of ``x`` ``[T, heads * head_dim]``; the other heads are
+    copied.  Returns new rows (``elementwise.rope`` is the in-place form for whole heads in the half layout)."""
+    _check_rows(x, "rotary")
+    _check(x, pos, table, n_rot_heads, 0, head_dim, None, None, "rotary")
+    return _QKNormRopeFn.apply(x, None, None, pos, table, n_rot_heads, 0, head_dim, 0.0, bool(interleaved))
+
+
+def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, pos: torch.Tensor, table: torch.Tensor,
+                 nq: int, nkv: int, head_dim: int, eps: float, interleaved: bool = False) -> torch.Tensor:
+    """RMS norm of every query head (weight ``q_norm`` ``[head_dim]``) and key head (``k_norm``) of ``qkv``
+    ``[T, (nq + nkv + ...) * head_dim]``, then the rotation; what lies behind the key heads is copied.  Returns new rows.
+    Weight gradients go to ``main_grad`` where the weights have one; they are summed in a fixed order."""
+    _check_rows(qkv, "qk_norm_rope")
+    if q_norm is None or k_norm is None:
+        raise ValueError("qk_norm_rope: both norm weights are needed (rotary() rotates without norms)")
+    _check(qkv, pos, table, nq, nkv, head_dim, q_norm, k_norm, "qk_norm_rope")
+    if q_norm.dtype != qkv.dtype or k_norm.dtype != qkv.dtype:
+        raise ValueError("qk_norm_rope: norm weights must have the rows' type")
+    return _QKNormRopeFn.apply(qkv, q_norm, k_norm, pos, table, nq, nkv, head_dim, float(eps), bool(interleaved))
+
+
+def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  slots: torch.Tensor, nq: int, nkv: int, head_dim: int, q_norm: torch.Tensor | None = None,
+                  k_norm: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows of a fused QKV projection on their way into attention, in one launch and without gradients: norms (when the
+    weights are given), rotation, and the key and value heads of row ``t`` written to cache slot ``slots[t]`` (a slot
+    outside the cache, such as -1, writes nothing; two rows must not share a slot).
+
+    ``x``: ``[T, (nq + 2 nkv) * head_dim]`` in the caches' type, or the fp32 partial sums ``[P, T, ...]`` of a split
+    projection, which are summed and rounded to that type first.  Caches: ``[blocks, block_size, nkv, head_dim]``.
+    Returns the rows, in ``out`` when given; ``out`` may be ``x`` itself."""
+    what = "qk_rope_cache"
+    if x.dim() not in (2, 3):
+        raise ValueError(f"{what}: rows must be [T, width] or partial sums [P, T, width], got {tuple(x.shape)}")
+    partial = x.dim() == 3
+    dt = k_cache.dtype
+    if dt not in _DTYPE or v_cache.dtype != dt or x.dtype != (torch.float32 if partial else dt):
+        raise ValueError(f"{what}: rows {x.dtype} and caches {dt}, {v_cache.dtype} do not go together")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError(f"{what} has no gradient: use qk_norm_rope or rotary where one is needed")
+    _check(x, pos, table, nq, nkv, head_dim, q_norm, k_norm, what)
+    T, W = x.shape[-2:]
+    if nkv < 1 or W != (nq + 2 * nkv) * head_dim:
+        raise ValueError(f"{what}: rows of width {W} are not {nq} query, {nkv} key and {nkv} value heads")
+    if partial and (x.shape[0] < 1 or x.stride(2) != 1 or (T > 1 and x.stride(1) < W)):
+        raise ValueError(f"{what}: partial sums must be rows of unit stride")
+    if q_norm is not None and (q_norm.dtype != dt or k_norm.dtype != dt):
+        raise ValueError(f"{what}: norm weights must have the caches' type")
+    if k_cache.shape != v_cache.shape or k_cache.shape[2:] != (nkv, head_dim):
+        raise ValueError(f"{what}: caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} do not hold {nkv} heads of size {head_dim}")
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous() or k_cache.dim() != 4:
+        raise ValueError(f"{what}: caches must be contiguous [blocks, block_size, heads, head_dim] tensors")
+    if slots.dtype != torch.int32 or slots.shape != (T,) or not slots.is_contiguous():
+        raise ValueError(f"{what}: slots must be a contiguous int32 [{T}] tensor")
+    if not (k_cache.device == v_cache.device == slots.device == x.device):
+        raise ValueError(f"{what}: rows, slots and caches must be on one device")
+    if out is not None and (out.shape != (T, W) or out.dtype != dt or out.device != x.device or out.stride(1) != 1
+                            or (T > 1 and out.stride(0) < W)):
+        raise ValueError(f"{what}: out must be [{T}, {W}] rows in the caches' type")
+    if not x.is_cuda:
+        rows = x.sum(0).to(dt) if partial else x
+        res = _fwd_ref(rows, q_norm, k_norm, pos, table, nq, nkv, head_dim, eps, interleaved, 1.0)
+        keep = (slots >= 0) & (slots < k_cache.shape[0] * k_cache.shape[1])
+        at = slots[keep].long()
+        k_cache.view(-1, nkv * head_dim)[at] = res[keep, nq * head_dim : (nq + nkv) * head_dim]
+        v_cache.view(-1, nkv * head_dim)[at] = res[keep, (nq + nkv) * head_dim :]
+        return res if out is None else out.copy_(res)
+    if not partial and (out is None or out.data_ptr() != x.data_ptr()):
+        x = _row_major(x)
+    if out is None:
+        out = torch.empty((T, W), device=x.device, dtype=dt)
+    elif out.data_ptr() == x.data_ptr() and not partial and out.stride() != x.stride() and T > 1:
+        raise ValueError(f"{what}: out lies on x with other strides")
+    return _launch_fwd(x, out, q_norm, k_norm, pos, table, nq, nkv, head_dim, float(eps), bool(interleaved), 1.0,
+                       x.shape[0] if partial else 0, slots, k_cache, v_cache)
