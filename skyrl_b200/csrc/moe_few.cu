@@ -13,6 +13,8 @@
 // Every result is summed in a fixed order, without atomics on floats.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "host_common.h"
 #include "ptx.cuh"
 
@@ -56,32 +58,58 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
   const int rank = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = static_cast<int>(blockIdx.x / kCluster) * kTok;
-  pdl_launch_dependents();
-  pdl_wait();
-  cluster.sync();  // every CTA of the cluster runs before its shared memory is written
+  cluster.barrier_arrive();
+  bool waited = false;
   const int per = (E + kCluster - 1) / kCluster;
   const int e_hi = min(E, (rank + 1) * per);
-  for (int e = rank * per + warp; e < e_hi; e += kWarps) {
-    const uint4* r = reinterpret_cast<const uint4*>(rw + static_cast<size_t>(e) * H);
-    double acc[kTok];
+  const int nv = H >> 3;
+  for (int e = rank * per + warp; e < e_hi; e += 2 * kWarps) {  // two experts at a time: their rows are all under way at once
+    const bool two = e + kWarps < e_hi;
+    const uint4* r0 = reinterpret_cast<const uint4*>(rw + static_cast<size_t>(e) * H);
+    const uint4* r1 = reinterpret_cast<const uint4*>(rw + static_cast<size_t>(two ? e + kWarps : e) * H);
+    double acc[2][kTok];
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) acc[i] = 0.0;
-#pragma unroll 4
-    for (int v = lane; v < (H >> 3); v += 32) {
-      const uint4 a = __ldg(r + v);
+    for (int i = 0; i < kTok; ++i) acc[0][i] = acc[1][i] = 0.0;
+    constexpr int kUnroll = kTok == 1 ? 8 : 4;
+    for (int v0 = lane; v0 < nv; v0 += 32 * kUnroll) {
+      uint4 a[kUnroll], b[kUnroll];
 #pragma unroll
-      for (int i = 0; i < kTok; ++i)
-        if (t0 + i < T)
-          acc[i] += static_cast<double>(
-              dot8(a, __ldg(reinterpret_cast<const uint4*>(h + static_cast<size_t>(t0 + i) * h_stride) + v)));
+      for (int j = 0; j < kUnroll; ++j) {
+        const int v = v0 + 32 * j;
+        a[j] = v < nv ? __ldg(r0 + v) : make_uint4(0, 0, 0, 0);
+        b[j] = v < nv ? __ldg(r1 + v) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j) {
+        const int v = v0 + 32 * j;
+#pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+          if (v >= nv || t0 + i >= T) continue;
+          const uint4 x = __ldg(reinterpret_cast<const uint4*>(h + static_cast<size_t>(t0 + i) * h_stride) + v);
+          acc[0][i] += static_cast<double>(dot8(a[j], x));
+          acc[1][i] += static_cast<double>(dot8(b[j], x));
+        }
+      }
     }
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
+    for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-      if (lane == 0) cluster.map_shared_rank(logits, i)[e] = acc[i];
+      for (int i = 0; i < kTok; ++i) {
+        acc[0][i] += __shfl_xor_sync(0xffffffffu, acc[0][i], o);
+        acc[1][i] += __shfl_xor_sync(0xffffffffu, acc[1][i], o);
+      }
+    if (!waited) cluster.barrier_wait();  // every CTA of the cluster runs before its shared memory is written
+    waited = true;
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) {
+        double* dst = cluster.map_shared_rank(logits, i);
+        dst[e] = acc[0][i] + 0.0;  // -0 counts as +0
+        if (two) dst[e + kWarps] = acc[1][i] + 0.0;
+      }
     }
   }
+  if (!waited) cluster.barrier_wait();
   cluster.sync();
   const int t = t0 + rank;
   if (rank >= kTok || t >= T || warp != 0) return;
@@ -92,45 +120,49 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
     }
     return;
   }
-  // k rounds of a warp-wide maximum; ties go to the lower expert.  A NaN counts as the smallest value, so that the
-  // indices stay in range, and makes the row's weights NaN.
-  const double inf = __longlong_as_double(0x7ff0000000000000ll);
-  uint32_t taken = 0;  // expert lane + 32 j: bit j
+  // k rounds of a warp-wide maximum over order-preserving 64-bit keys, the high words first.  A lane keeps the best of
+  // its experts lane + 32 j and looks again only after it has lost it.  Ties go to the lower expert.  A NaN counts as
+  // the smallest value, so that the indices stay in range, and makes the row's weights NaN.
+  uint32_t taken = 0;  // bit j: expert lane + 32 j
   bool bad = false;
+  unsigned long long best = 0;
+  int best_e = 0x7fffffff;
+  auto look = [&]() {
+    best = 0;
+    best_e = 0x7fffffff;
+    for (int j = 0, e = lane; e < E; ++j, e += 32) {
+      const double v = logits[e];
+      const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
+      const bool nan = v != v;
+      bad |= nan;
+      const unsigned long long key = nan ? 0ull : (b >> 63 ? ~b : b | 0x8000000000000000ull);
+      if (!(taken >> j & 1) && (best_e == 0x7fffffff || key > best)) {
+        best = key;
+        best_e = e;
+      }
+    }
+  };
+  look();
   double top = 0.0;
   float mine = 0.f, sel = 0.f;
   int my_e = 0;
   for (int s = 0; s < k; ++s) {
-    double best = -inf;
-    int best_e = 0x7fffffff;
-    for (int j = 0, e = lane; e < E; ++j, e += 32) {
-      if (taken >> j & 1) continue;
-      double v = logits[e];
-      if (v != v) {
-        bad = true;
-        v = -inf;
-      }
-      if (v > best || best_e == 0x7fffffff) {
-        best = v;
-        best_e = e;
-      }
+    const bool have = best_e != 0x7fffffff;
+    const uint32_t hi = have ? static_cast<uint32_t>(best >> 32) : 0u, lo = have ? static_cast<uint32_t>(best) : 0u;
+    const uint32_t top_hi = __reduce_max_sync(0xffffffffu, hi);
+    const uint32_t top_lo = __reduce_max_sync(0xffffffffu, hi == top_hi ? lo : 0u);
+    const uint32_t win = __reduce_min_sync(0xffffffffu, have && hi == top_hi && lo == top_lo ? static_cast<uint32_t>(best_e) : 0x7fffffffu);
+    if (have && best_e == static_cast<int>(win)) {
+      taken |= 1u << (win >> 5);
+      look();
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double ov = __shfl_xor_sync(0xffffffffu, best, o);
-      const int oe = __shfl_xor_sync(0xffffffffu, best_e, o);
-      if (oe != 0x7fffffff && (best_e == 0x7fffffff || ov > best || (ov == best && oe < best_e))) {
-        best = ov;
-        best_e = oe;
-      }
-    }
-    if ((best_e & 31) == lane) taken |= 1u << (best_e >> 5);
-    if (s == 0) top = best;
-    const float p = expf(static_cast<float>(best - top));
+    const double v = logits[win];
+    if (s == 0) top = v;
+    const float p = expf(static_cast<float>(v - top));
     sel += p;
     if (lane == s) {
       mine = p;
-      my_e = best_e;
+      my_e = static_cast<int>(win);
     }
   }
   float all = sel;
@@ -147,55 +179,123 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
 }
 
 // ---------------------------------------------------------------------------
-// Rows of every expert, in shared memory: entry = token * k + slot.  The order of an expert's entries does not matter
-// (an entry's result does not depend on its neighbours).
+// Rows of every expert, in shared memory: entry = token * k + slot.  An expert's rows are taken in units of at most
+// kUnitRows.  An entry's result does not depend on its neighbours, so the order of an expert's entries matters only where
+// they are cut into units, which all CTAs have to cut alike.
 // ---------------------------------------------------------------------------
+constexpr int kUnitRows = 16;
+
 struct Lists {
-  int first[kMaxExperts + 1];         // first entry of each expert
-  int cursor[kMaxExperts];
-  unsigned short used[kMaxExperts];   // experts that have entries, ascending
-  unsigned short entry[kMaxEntries];
-  int n_used;
+  int* cursor;              // [E] scratch of the construction
+  unsigned short* first;    // [E + 1] first entry of each expert
+  unsigned short* used;     // [E] experts that have entries, ascending
+  unsigned short* unit0;    // [E + 1] first unit of the i-th used expert
+  unsigned short* entry;    // [n]
+  int* count;               // used experts, units, rows of the largest unit
+  int n_used, n_units, most;
 };
 
-__device__ __forceinline__ void build_lists(Lists& L, const int* __restrict__ idx, int n, int E) {
-  for (int e = threadIdx.x; e < E; e += kThreads) L.cursor[e] = 0;
+__host__ __device__ constexpr int lists_bytes(int n, int E) { return (4 * E + 2 * (E + 1) * 2 + 2 * E + 2 * n + 16 + 127) / 128 * 128; }
+
+__device__ __forceinline__ Lists build_lists(char* smem, const int* __restrict__ idx, int n, int E) {
+  Lists L;
+  L.count = reinterpret_cast<int*>(smem);
+  L.cursor = L.count + 4;
+  L.first = reinterpret_cast<unsigned short*>(L.cursor + E);
+  L.unit0 = L.first + E + 1;
+  L.used = L.unit0 + E + 1;
+  L.entry = L.used + E;
+  for (int e = threadIdx.x; e < E; e += blockDim.x) L.cursor[e] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int e = idx[i];
     if (e >= 0 && e < E) atomicAdd(&L.cursor[e], 1);
   }
   __syncthreads();
   if (threadIdx.x < 32) {
-    int run = 0, used = 0;
+    const int lane = threadIdx.x;
+    int run = 0, used = 0, units = 0, most = 0;
     for (int base = 0; base < E; base += 32) {
-      const int e = base + threadIdx.x;
+      const int e = base + lane;
       const int c = e < E ? L.cursor[e] : 0;
-      int inc = c;
+      // rows in the low half, units in the high half: neither passes 16 bits (at most kMaxEntries of each)
+      int inc = c | ((c + kUnitRows - 1) / kUnitRows) << 16;
+      const int own = inc;
+      most = max(most, c);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (threadIdx.x >= o) inc += v;
+        if (lane >= o) inc += v;
       }
       const unsigned int has = __ballot_sync(0xffffffffu, c > 0);
       if (e < E) {
-        L.first[e] = L.cursor[e] = run + inc - c;
-        if (c > 0) L.used[used + __popc(has & ((1u << threadIdx.x) - 1u))] = static_cast<unsigned short>(e);
+        L.cursor[e] = run + ((inc - own) & 0xffff);
+        L.first[e] = static_cast<unsigned short>(L.cursor[e]);
+        if (c > 0) {
+          const int a = used + __popc(has & ((1u << lane) - 1u));
+          L.used[a] = static_cast<unsigned short>(e);
+          L.unit0[a] = static_cast<unsigned short>(units + ((inc - own) >> 16));
+        }
       }
-      run += __shfl_sync(0xffffffffu, inc, 31);
+      const int tot = __shfl_sync(0xffffffffu, inc, 31);
+      run += tot & 0xffff;
+      units += tot >> 16;
       used += __popc(has);
     }
-    if (threadIdx.x == 0) {
-      L.first[E] = run;
-      L.n_used = used;
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) {
+      L.first[E] = static_cast<unsigned short>(run);
+      L.unit0[used] = static_cast<unsigned short>(units);
+      L.count[0] = used;
+      L.count[1] = units;
+      L.count[2] = min(most, kUnitRows);
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int e = idx[i];
-    if (e >= 0 && e < E) L.entry[atomicAdd(&L.cursor[e], 1)] = static_cast<unsigned short>(i);
+  L.n_used = L.count[0];
+  L.n_units = L.count[1];
+  L.most = L.count[2];
+  if (L.n_units == L.n_used) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int e = idx[i];
+      if (e >= 0 && e < E) L.entry[atomicAdd(&L.cursor[e], 1)] = static_cast<unsigned short>(i);
+    }
+  } else if (threadIdx.x < 32) {  // in the entries' order, 32 at a time
+    const int lane = threadIdx.x;
+    for (int base = 0; base < n; base += 32) {
+      const int i = base + lane;
+      int e = i < n ? idx[i] : -1;
+      const bool on = e >= 0 && e < E;
+      if (!on) e = -1 - lane;
+      const unsigned int peers = __match_any_sync(0xffffffffu, e);
+      const int rank = __popc(peers & ((1u << lane) - 1u));
+      if (on) L.entry[L.cursor[e] + rank] = static_cast<unsigned short>(i);
+      __syncwarp();
+      if (on && rank == 0) L.cursor[e] += __popc(peers);
+      __syncwarp();
+    }
   }
   __syncthreads();
+  return L;
+}
+
+struct Unit {
+  int e, r0, r1;  // expert and its entries [r0, r1)
+};
+__device__ __forceinline__ Unit unit_at(const Lists& L, int unit) {
+  int lo = 0, hi = L.n_used - 1;  // last used expert whose first unit is not behind `unit`
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (L.unit0[mid] <= unit)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  Unit u;
+  u.e = L.used[lo];
+  u.r0 = L.first[u.e] + (unit - L.unit0[lo]) * kUnitRows;
+  u.r1 = min(static_cast<int>(L.first[u.e + 1]), u.r0 + kUnitRows);
+  return u;
 }
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -204,29 +304,300 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// weights are read once: keep them from displacing the rows in L1
+
+// ---------------------------------------------------------------------------
+// The weight stream.  An item is 16 weight rows of one unit, in two blocks of eight rows that lie one behind the other in
+// memory.  A ring of stages takes a block each (or a piece of at most kMaxPiece columns of it); one lane fills it with
+// bulk copies as far ahead as the ring is long, a whole block in a copy where it fits: a copy costs the engine about 90
+// cycles whatever its size, so that rows of 1.5 KB one by one would come at 4.8 TB/s and 12 KB blocks come at 6.7.
+// Eight warps take a share of every piece's columns each; their sums meet in shared memory at the end of the item.
+// ---------------------------------------------------------------------------
+constexpr int kConsumers = 8;
+constexpr int kConsumerThreads = 32 * kConsumers;
+constexpr int kRingThreads = kConsumerThreads + 32;
+constexpr int kMaxStages = 24;
+constexpr int kMaxPiece = 2048;  // columns; a warp's share is at most 8 k steps of 32
+constexpr int kMaxNt = kUnitRows / 8;
+constexpr int kRedBytes = 2 * kConsumers * kMaxNt * 32 * 16;  // sums of two items
+
+struct Ring {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+};
+
+struct Shape {
+  int stages, pieces, piece, K;  // piece: columns of a stage's rows
+};
+
+struct Turn {  // place in the ring
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void step(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+// Weights that other kernels wrote through ordinary stores are read by bulk copies.
+__device__ __forceinline__ void fence_proxy_async_global() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumerThreads) : "memory"); }
+
+// Fill the stages of one item (called by a whole warp): blocks of rows_a rows at a and rows_b rows at b.  Returns false
+// when a wait gave up.
+__device__ __forceinline__ bool produce_item(Ring& ring, char* buf, const Shape& s, Turn& turn, const __nv_bfloat16* a, int rows_a,
+                                             const __nv_bfloat16* b, int rows_b, int* status) {
+  const int lane = threadIdx.x & 31;
+  for (int q = 0; q < s.pieces; ++q)
+    for (int half = 0; half < 2; ++half, turn.step(s.stages)) {
+      const __nv_bfloat16* src = half ? b : a;
+      const int rows = half ? rows_b : rows_a;
+      if (!mbar_wait(&ring.empty[turn.stage], turn.parity ^ 1, status, 0x4d01)) return false;
+      const uint32_t bytes = 2u * min(s.piece, s.K - q * s.piece);
+      char* dst = buf + static_cast<size_t>(turn.stage) * 16 * s.piece;
+      if (lane == 0) mbar_arrive_expect_tx(&ring.full[turn.stage], bytes * rows);
+      __syncwarp();
+      if (s.pieces == 1) {
+        if (lane == 0 && rows > 0) bulk_load(dst, src, bytes * rows, &ring.full[turn.stage]);
+      } else if (lane < rows) {
+        bulk_load(dst + lane * 2 * s.piece, src + static_cast<size_t>(lane) * s.K + q * s.piece, bytes, &ring.full[turn.stage]);
+      }
+    }
+  return true;
+}
+
+// The consumers' loop over `items` items.  unit_of() gives the unit of the next item, row_ptr(r) the operand row of entry
+// r, finish(unit, sums) takes the warps' sums [warp][column group][lane] of an item.  A warp's share of the operand rows
+// stays in registers from item to item of a unit (rows of more than one piece: from L1 or L2 again).
+template <int kNt, int kSteps, class UnitOf, class RowPtr, class Finish>
+__device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red, const Shape& s, int items, int* status,
+                                        UnitOf unit_of, RowPtr row_ptr, Finish finish) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  // k steps of piece q that fall to this warp: `mine` from `lo`; the first `some` of them have columns for this lane
+  int lo = 0, mine = 0, some = 0;
+  auto share = [&](int q) {
+    const int cols = min(s.piece, s.K - q * s.piece);
+    const int steps = (cols + 31) >> 5;
+    lo = warp * steps / kConsumers;
+    mine = (warp + 1) * steps / kConsumers - lo;
+    some = min(mine, max(0, (cols - lo * 32 - 8 * t4 + 31) >> 5));
+  };
+  share(0);
+  const __nv_bfloat16* x[kNt];
+  uint4 v[kSteps][kNt];
+  auto request = [&](int q) {
+    const int at = q * s.piece + lo * 32;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+        v[j][n] = j < some && x[n] ? *reinterpret_cast<const uint4*>(x[n] + at + j * 32) : make_uint4(0, 0, 0, 0);
+  };
+  Turn turn;
+  int r0 = -1;
+  for (int i = 0; i < items; ++i) {
+    const Unit u = unit_of();
+    float acc[kNt][4];
+#pragma unroll
+    for (int n = 0; n < kNt; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[n][c] = 0.f;
+    const bool changed = u.r0 != r0;
+    if (changed) {
+      r0 = u.r0;
+#pragma unroll
+      for (int n = 0; n < kNt; ++n) {
+        const int r = r0 + n * 8 + g;
+        x[n] = r < u.r1 ? row_ptr(r) + 8 * t4 : nullptr;
+      }
+    }
+    for (int q = 0; q < s.pieces; ++q) {
+      if (s.pieces > 1) share(q);
+      if (changed || s.pieces > 1) request(q);
+      const int off = g * 2 * s.piece + lo * 64 + 16 * t4;
+      const char* top = buf + static_cast<size_t>(turn.stage) * 16 * s.piece + off;
+      uint64_t* free_a = &ring.empty[turn.stage];
+      if (!mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d02)) return;
+      turn.step(s.stages);
+      const char* low = buf + static_cast<size_t>(turn.stage) * 16 * s.piece + off;
+      uint64_t* free_b = &ring.empty[turn.stage];
+      if (!mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d03)) return;
+      turn.step(s.stages);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        if (j >= mine) break;
+        uint4 a = make_uint4(0, 0, 0, 0), b = a;
+        if (j < some) {  // what lies behind a row in a stage belongs to other rows
+          a = *reinterpret_cast<const uint4*>(top + j * 64);
+          b = *reinterpret_cast<const uint4*>(low + j * 64);
+        }
+#pragma unroll
+        for (int n = 0; n < kNt; ++n) {
+          mma_bf16(acc[n], a.x, b.x, a.y, b.y, v[j][n].x, v[j][n].y);
+          mma_bf16(acc[n], a.z, b.z, a.w, b.w, v[j][n].z, v[j][n].w);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(free_a);
+        mbar_arrive(free_b);
+      }
+    }
+    // two buffers: an item's sums are read while the next item's are not yet all written, so one barrier an item is enough
+    float4* sums = red + (i & 1) * (kConsumers * kNt * 32);
+#pragma unroll
+    for (int n = 0; n < kNt; ++n) sums[(warp * kNt + n) * 32 + lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+    consumer_sync();
+    finish(u, sums);
+  }
+}
+
+// Sum over the warps of component c of column group n's fragment in lane l.
+template <int kNt>
+__device__ __forceinline__ float warp_total(const float4* sums, int n, int l, int c) {
+  float v = 0.f;
+#pragma unroll
+  for (int w = 0; w < kConsumers; ++w) v += reinterpret_cast<const float*>(&sums[(w * kNt + n) * 32 + l])[c];
+  return v;
+}
+
+__device__ __forceinline__ void ring_init(Ring& ring, int stages) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&ring.full[i], 1);
+      mbar_init(&ring.empty[i], kConsumers);
+    }
+    fence_mbar_init();
+  }
+}
+// After a wait gave up: let the copies that are still under way land before the CTA's shared memory is given back.
+__device__ __forceinline__ void ring_drain(Ring& ring, const Shape& s, Turn turn) {
+  for (int i = 0; i < s.stages; ++i, turn.step(s.stages)) {  // from the oldest stage on; a stage never filled waits in vain
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(&ring.full[turn.stage], turn.parity ^ 1))
+      if (globaltimer_ns() - t0 > kWaitTimeoutNs / 100) break;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Gate and up projections: an item is eight gate rows and the eight up rows beside them, so that a lane holds both
+// factors of an activation.
+// ---------------------------------------------------------------------------
+template <int kSteps>
+__global__ void __launch_bounds__(kRingThreads, 1)
+gate_up_kernel(const __nv_bfloat16* h, long long h_stride, const int* __restrict__ idx, const __nv_bfloat16* __restrict__ wgu,
+               __nv_bfloat16* act, int n, int k, int E, int H, int F, Shape s, int* status) {
+  __shared__ Ring ring;
+  extern __shared__ __align__(128) char smem[];
+  float4* red = reinterpret_cast<float4*>(smem);
+  char* buf = smem + kRedBytes;
+  ring_init(ring, s.stages);
+  const Lists L = build_lists(buf + static_cast<size_t>(s.stages) * 16 * s.piece, idx, n, E);
+  const int tiles = (F + 7) >> 3;
+  const long long items = static_cast<long long>(L.n_units) * tiles;
+  const int lo = static_cast<int>(items * blockIdx.x / gridDim.x), hi = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
+  if (threadIdx.x >= kConsumerThreads) {
+    Turn turn;
+    int unit = lo / tiles, tile = lo - unit * tiles;
+    fence_proxy_async_global();
+    for (int i = lo; i < hi; ++unit, tile = 0) {
+      const Unit u = unit_at(L, unit);
+      for (; tile < tiles && i < hi; ++tile, ++i) {
+        const int f0 = tile * 8, rows = min(8, F - f0);
+        const __nv_bfloat16* w = wgu + (static_cast<size_t>(u.e) * 2 * F + f0) * H;
+        if (!produce_item(ring, buf, s, turn, w, rows, w + static_cast<size_t>(F) * H, rows, status)) {
+          ring_drain(ring, s, turn);
+          return;
+        }
+      }
+    }
+    return;
+  }
+  auto run = [&](auto nt) {
+    constexpr int kNt = decltype(nt)::value;
+    int unit = lo / tiles, tile = lo - unit * tiles - 1, f0 = 0;
+    Unit u = {};
+    if (lo < hi) u = unit_at(L, unit);
+    auto unit_of = [&]() {
+      if (++tile == tiles) {
+        tile = 0;
+        u = unit_at(L, ++unit);
+      }
+      f0 = tile * 8;
+      return u;
+    };
+    auto row_ptr = [&](int r) { return h + static_cast<size_t>(L.entry[r] / k) * h_stride; };
+    auto finish = [&](const Unit& v, const float4* sums) {
+      const int o = threadIdx.x;  // (column group, lane of the fragment, one of its two columns)
+      if (o >= kNt * 64) return;
+      const int c = o & 1, l = (o >> 1) & 31, grp = o >> 6;
+      const int r = v.r0 + grp * 8 + 2 * (l & 3) + c, f = f0 + (l >> 2);
+      if (r >= v.r1 || f >= F) return;
+      const float gate = warp_total<kNt>(sums, grp, l, c), up = warp_total<kNt>(sums, grp, l, 2 + c);
+      // the activation is the down product's bf16 operand, rounded here as on the path for many tokens
+      act[static_cast<size_t>(L.entry[r]) * F + f] = __float2bfloat16_rn(gate / (1.f + __expf(-gate)) * up);
+    };
+    consume<kNt, kSteps>(ring, buf, red, s, hi - lo, status, unit_of, row_ptr, finish);
+  };
+  if (L.most <= 8)
+    run(std::integral_constant<int, 1>());
+  else
+    run(std::integral_constant<int, 2>());
+}
+
+// ---------------------------------------------------------------------------
+// Down projection and combination.  A CTA owns 16 columns of the output for all tokens.  Its warps take the units in turn,
+// one each, with the weights straight from global memory into fragments: 16 warps with 16 loads a lane keep 128 KB a SM
+// under way, and no warp waits for another.  The entries' results stay in shared memory until all are there and are then
+// added up slot by slot, so no sum crosses a CTA.
+// ---------------------------------------------------------------------------
+constexpr int kDownThreads = 512;
+
+// weights are read once: keep them from displacing the operand rows in L1
 __device__ __forceinline__ uint4 ld_stream(const __nv_bfloat16* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 
-// acc[n] (+)= 16 weight rows x 8 kNt operand rows over the k steps [s0, s1) of 32.  top / low: this lane's two weight
-// rows (g and g + 8, null outside the matrix) at k = 8 (lane % 4); x[n]: its operand row of column group n.
-template <int kNt, int kUnroll>
-__device__ __forceinline__ void products(float (&acc)[kNt][4], const __nv_bfloat16* top, const __nv_bfloat16* low,
-                                         const __nv_bfloat16* const (&x)[kNt], int s0, int s1, int K, int t4) {
-  for (int s = s0; s < s1; s += kUnroll) {
+template <int kNt>
+__device__ __forceinline__ void down_unit(const Lists& L, float* y, const __nv_bfloat16* act, const __nv_bfloat16* wd, const Unit& u,
+                                          int n0, int H, int F) {
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  constexpr int kUnroll = kNt == 1 ? 8 : 4;
+  const __nv_bfloat16* base = wd + (static_cast<size_t>(u.e) * H + n0) * F + 8 * t4;
+  // rows behind the last are read as the last one; their results are not stored
+  const __nv_bfloat16* top = base + static_cast<size_t>(min(g, H - 1 - n0)) * F;
+  const __nv_bfloat16* low = base + static_cast<size_t>(min(g + 8, H - 1 - n0)) * F;
+  const __nv_bfloat16* x[kNt];
+  float acc[kNt][4];
+#pragma unroll
+  for (int n = 0; n < kNt; ++n) {
+    const int r = u.r0 + n * 8 + g;
+    x[n] = r < u.r1 ? act + static_cast<size_t>(L.entry[r]) * F + 8 * t4 : nullptr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+  }
+  const int steps = (F - 8 * t4 + 31) >> 5;  // of this lane; lane t4 = 0 has the most
+  const int all = (F + 31) >> 5;
+  for (int s = 0; s < all; s += kUnroll) {
     uint4 a[kUnroll], b[kUnroll], v[kUnroll][kNt];
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
-      const int col = (s + j) * 32;
-      const bool ok = s + j < s1 && col + 8 * t4 < K;
       const uint4 z = make_uint4(0, 0, 0, 0);
-      a[j] = ok && top ? ld_stream(top + col) : z;
-      b[j] = ok && low ? ld_stream(low + col) : z;
+      const bool ok = s + j < steps;
+      a[j] = ok ? ld_stream(top + (s + j) * 32) : z;
+      b[j] = ok ? ld_stream(low + (s + j) * 32) : z;
 #pragma unroll
-      for (int n = 0; n < kNt; ++n) v[j][n] = ok && x[n] ? *reinterpret_cast<const uint4*>(x[n] + col) : z;
+      for (int n = 0; n < kNt; ++n) v[j][n] = ok && x[n] ? *reinterpret_cast<const uint4*>(x[n] + (s + j) * 32) : z;
     }
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j)
@@ -236,110 +607,12 @@ __device__ __forceinline__ void products(float (&acc)[kNt][4], const __nv_bfloat
         mma_bf16(acc[n], a[j].z, b[j].z, a[j].w, b[j].w, v[j][n].z, v[j][n].w);
       }
   }
-}
-
-// ---------------------------------------------------------------------------
-// Gate and up projections.  An item is eight gate rows and the eight up rows beside them of one expert: a lane then
-// holds both factors of an activation.  The CTA's warps split K; their sums meet in shared memory.
-// ---------------------------------------------------------------------------
-constexpr int kMaxNt = 4;
-
-template <int kNt, int kUnroll>
-__device__ __forceinline__ void gate_up_tile(const Lists& L, float4* red, const __nv_bfloat16* h, long long h_stride,
-                                             const __nv_bfloat16* wgu, __nv_bfloat16* act, int e, int f0, int r0, int r1, int k,
-                                             int H, int F) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, t4 = lane & 3;
-  const int steps = (H + 31) >> 5;
-  const int s0 = warp * steps / kWarps, s1 = (warp + 1) * steps / kWarps;
-  const __nv_bfloat16* top = f0 + g < F ? wgu + (static_cast<size_t>(e) * 2 * F + f0 + g) * H + 8 * t4 : nullptr;
-  const __nv_bfloat16* low = top ? top + static_cast<size_t>(F) * H : nullptr;
-  const __nv_bfloat16* x[kNt];
-  float acc[kNt][4];
-#pragma unroll
-  for (int n = 0; n < kNt; ++n) {
-    const int r = r0 + n * 8 + g;
-    x[n] = r < r1 ? h + static_cast<size_t>(L.entry[r] / k) * h_stride + 8 * t4 : nullptr;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-  }
-  products<kNt, kUnroll>(acc, top, low, x, s0, s1, H, t4);
-#pragma unroll
-  for (int n = 0; n < kNt; ++n) red[(warp * kNt + n) * 32 + lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-  __syncthreads();
-  // thread -> (column group, lane of the fragment, one of its two columns)
-  for (int i = threadIdx.x; i < kNt * 64; i += kThreads) {
-    const int n = i >> 6, l = (i >> 1) & 31, col = i & 1;
-    const int r = r0 + n * 8 + 2 * (l & 3) + col, f = f0 + (l >> 2);
-    if (r >= r1 || f >= F) continue;
-    float gate = 0.f, up = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float* p = reinterpret_cast<const float*>(&red[(w * kNt + n) * 32 + l]);
-      gate += p[col];
-      up += p[2 + col];
-    }
-    // the activation is the down product's bf16 operand, rounded here as on the path for many tokens
-    act[static_cast<size_t>(L.entry[r]) * F + f] = __float2bfloat16_rn(gate / (1.f + __expf(-gate)) * up);
-  }
-}
-
-__global__ void __launch_bounds__(kThreads, 2)
-gate_up_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const int* __restrict__ idx,
-               const __nv_bfloat16* __restrict__ wgu, __nv_bfloat16* __restrict__ act, int n, int k, int E, int H, int F) {
-  __shared__ Lists L;
-  __shared__ float4 red[2][kWarps * kMaxNt * 32];
-  pdl_launch_dependents();
-  pdl_wait();
-  build_lists(L, idx, n, E);
-  const int tiles = (F + 7) >> 3;
-  const long long items = static_cast<long long>(L.n_used) * tiles;
-  const int lo = static_cast<int>(items * blockIdx.x / gridDim.x), hi = static_cast<int>(items * (blockIdx.x + 1) / gridDim.x);
-  int flip = 0;
-  for (int i = lo; i < hi; ++i) {
-    const int e = L.used[i / tiles], f0 = (i % tiles) * 8;
-    const int r1 = L.first[e + 1];
-    for (int r0 = L.first[e]; r0 < r1; r0 += 8 * kMaxNt, flip ^= 1) {
-      const int m = r1 - r0;
-      if (m <= 8)
-        gate_up_tile<1, 8>(L, red[flip], h, h_stride, wgu, act, e, f0, r0, r1, k, H, F);
-      else if (m <= 16)
-        gate_up_tile<2, 4>(L, red[flip], h, h_stride, wgu, act, e, f0, r0, r1, k, H, F);
-      else
-        gate_up_tile<4, 2>(L, red[flip], h, h_stride, wgu, act, e, f0, r0, min(r1, r0 + 32), k, H, F);
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Down projection and combination.  A CTA owns 16 columns of the output for all tokens and walks over the used experts,
-// one expert a warp at a time; the entries' results stay in shared memory until all are there and are then added up
-// slot by slot, so no sum crosses a CTA.
-// ---------------------------------------------------------------------------
-template <int kNt, int kUnroll>
-__device__ __forceinline__ void down_tile(const Lists& L, float* y, const __nv_bfloat16* act, const __nv_bfloat16* wd, int e,
-                                          int n0, int r0, int r1, int H, int F) {
-  const int lane = threadIdx.x & 31;
-  const int g = lane >> 2, t4 = lane & 3;
-  const __nv_bfloat16* base = wd + (static_cast<size_t>(e) * H + n0) * F + 8 * t4;
-  const __nv_bfloat16* top = n0 + g < H ? base + static_cast<size_t>(g) * F : nullptr;
-  const __nv_bfloat16* low = n0 + g + 8 < H ? base + static_cast<size_t>(g + 8) * F : nullptr;
-  const __nv_bfloat16* x[kNt];
-  float acc[kNt][4];
-#pragma unroll
-  for (int n = 0; n < kNt; ++n) {
-    const int r = r0 + n * 8 + g;
-    x[n] = r < r1 ? act + static_cast<size_t>(L.entry[r]) * F + 8 * t4 : nullptr;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-  }
-  products<kNt, kUnroll>(acc, top, low, x, 0, (F + 31) >> 5, F, t4);
 #pragma unroll
   for (int n = 0; n < kNt; ++n)
 #pragma unroll
     for (int col = 0; col < 2; ++col) {
-      const int r = r0 + n * 8 + 2 * t4 + col;
-      if (r < r1) {
+      const int r = u.r0 + n * 8 + 2 * t4 + col;
+      if (r < u.r1) {
         float* o = y + L.entry[r] * 16;
         o[g] = acc[n][col];
         o[g + 8] = acc[n][2 + col];
@@ -347,39 +620,74 @@ __device__ __forceinline__ void down_tile(const Lists& L, float* y, const __nv_b
     }
 }
 
-__global__ void __launch_bounds__(kThreads)
-down_kernel(const __nv_bfloat16* __restrict__ act, const int* __restrict__ idx, const float* __restrict__ w,
-            const __nv_bfloat16* __restrict__ wd, __nv_bfloat16* __restrict__ out, int T, int k, int E, int H, int F) {
-  __shared__ Lists L;
-  extern __shared__ float y[];  // [T * k][16]
-  pdl_launch_dependents();
-  pdl_wait();
+__global__ void __launch_bounds__(kDownThreads, 1)
+down_kernel(const __nv_bfloat16* act, const int* __restrict__ idx, const float* w, const __nv_bfloat16* __restrict__ wd,
+            __nv_bfloat16* __restrict__ out, int T, int k, int E, int H, int F) {
+  extern __shared__ __align__(128) char smem[];
   const int n = T * k;
-  build_lists(L, idx, n, E);
+  float* y = reinterpret_cast<float*>(smem);  // [n][16]
+  const Lists L = build_lists(smem + sizeof(float) * 16 * static_cast<size_t>(n), idx, n, E);
   const int n0 = blockIdx.x * 16;
-  for (int a = threadIdx.x >> 5; a < L.n_used; a += kWarps) {
-    const int e = L.used[a], r1 = L.first[e + 1];
-    for (int r0 = L.first[e]; r0 < r1; r0 += 8 * kMaxNt) {
-      const int m = r1 - r0;
-      if (m <= 8)
-        down_tile<1, 8>(L, y, act, wd, e, n0, r0, r1, H, F);
-      else if (m <= 16)
-        down_tile<2, 4>(L, y, act, wd, e, n0, r0, r1, H, F);
-      else
-        down_tile<4, 2>(L, y, act, wd, e, n0, r0, min(r1, r0 + 32), H, F);
-    }
+  for (int i = threadIdx.x >> 5; i < L.n_units; i += kDownThreads / 32) {
+    const Unit u = unit_at(L, i);
+    if (u.r1 - u.r0 <= 8)
+      down_unit<1>(L, y, act, wd, u, n0, H, F);
+    else
+      down_unit<2>(L, y, act, wd, u, n0, H, F);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < T * 16; i += kThreads) {
+  for (int i = threadIdx.x; i < T * 16; i += kDownThreads) {
     const int t = i >> 4, c = i & 15;
     if (n0 + c >= H) continue;
     float v = 0.f;
-    for (int s = 0; s < k; ++s) {
-      const int e = idx[t * k + s];
-      if (e >= 0 && e < E) v = fmaf(w[t * k + s], y[(t * k + s) * 16 + c], v);
+    for (int j = 0; j < k; ++j) {
+      const int e = idx[t * k + j];
+      if (e >= 0 && e < E) v = fmaf(w[t * k + j], y[(t * k + j) * 16 + c], v);
     }
     out[static_cast<size_t>(t) * H + n0 + c] = __float2bfloat16_rn(v);
   }
+}
+
+// Stages of eight rows of K columns in `room` bytes.  A row of more than kMaxPiece columns comes in equal pieces.
+inline Shape ring_shape(int K, size_t room) {
+  Shape s;
+  s.K = K;
+  s.pieces = (K + kMaxPiece - 1) / kMaxPiece;
+  s.piece = s.pieces == 1 ? K : ((K + s.pieces - 1) / s.pieces + 31) / 32 * 32;
+  const size_t fit = room / (16 * static_cast<size_t>(s.piece));
+  s.stages = static_cast<int>(fit < kMaxStages ? fit : kMaxStages);
+  return s;
+}
+
+template <int kSteps>
+cudaError_t launch_gate_up(const void* h, long long h_stride, const int* idx, const void* wgu, void* act, int T, int k, int E, int H,
+                           int F, const Shape& s, size_t smem, size_t smem_most, int* status, cudaStream_t st) {
+  static bool attr_dev[64] = {};
+  bool& attr = attr_dev[device_index()];
+  if (!attr) {
+    const cudaError_t e = cudaFuncSetAttribute(gate_up_kernel<kSteps>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_most));
+    if (e != cudaSuccess) return e;
+    attr = true;
+  }
+  gate_up_kernel<kSteps><<<sm_count(), kRingThreads, smem, st>>>(static_cast<const __nv_bfloat16*>(h), h_stride, idx,
+                                                                 static_cast<const __nv_bfloat16*>(wgu), static_cast<__nv_bfloat16*>(act),
+                                                                 T * k, k, E, H, F, s, status);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_down(const void* act, const int* idx, const float* w, const void* wd, void* out, int T, int k, int E, int H, int F,
+                        size_t smem, size_t smem_most, cudaStream_t st) {
+  static bool attr_dev[64] = {};
+  bool& attr = attr_dev[device_index()];
+  if (!attr) {
+    const cudaError_t e = cudaFuncSetAttribute(down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_most));
+    if (e != cudaSuccess) return e;
+    attr = true;
+  }
+  down_kernel<<<(H + 15) / 16, kDownThreads, smem, st>>>(static_cast<const __nv_bfloat16*>(act), idx, w,
+                                                         static_cast<const __nv_bfloat16*>(wd), static_cast<__nv_bfloat16*>(out), T, k,
+                                                         E, H, F);
+  return cudaGetLastError();
 }
 
 }  // namespace mf
@@ -398,14 +706,11 @@ int sb_moe_few_route(const void* h, long long h_stride, const void* router, cons
   const auto* hp = static_cast<const __nv_bfloat16*>(h);
   const auto* rp = static_cast<const __nv_bfloat16*>(router);
   // a token a cluster while the clusters fit the SMs side by side; beyond that four share the router's rows
-  cudaError_t e;
   if (T * sb::mf::kCluster <= sb::sm_count())
-    e = sb::launch_pdl(sb::mf::route_kernel<1>, dim3(T * sb::mf::kCluster), dim3(sb::mf::kThreads), smem, st, hp, h_stride, rp, live,
-                       w, idx, T, E, H, k, norm);
+    sb::mf::route_kernel<1><<<T * sb::mf::kCluster, sb::mf::kThreads, smem, st>>>(hp, h_stride, rp, live, w, idx, T, E, H, k, norm);
   else
-    e = sb::launch_pdl(sb::mf::route_kernel<4>, dim3((T + 3) / 4 * sb::mf::kCluster), dim3(sb::mf::kThreads), smem, st, hp, h_stride,
-                       rp, live, w, idx, T, E, H, k, norm);
-  return e == cudaSuccess ? SB_OK : SB_ERR_CUDA;
+    sb::mf::route_kernel<4><<<(T + 3) / 4 * sb::mf::kCluster, sb::mf::kThreads, smem, st>>>(hp, h_stride, rp, live, w, idx, T, E, H, k, norm);
+  return cudaGetLastError() == cudaSuccess ? SB_OK : SB_ERR_CUDA;
 }
 
 // h [T, H], idx int32 / w fp32 [T, k] (idx outside [0, E): the slot contributes nothing), wgu [E, 2F, H], wd [E, H, F];
@@ -419,22 +724,20 @@ int sb_moe_few_experts(const void* h, long long h_stride, const float* w, const 
        reinterpret_cast<uintptr_t>(act)) & 15)
     return SB_ERR_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  static bool attr_dev[64] = {};
-  bool& attr = attr_dev[sb::device_index()];
-  const size_t most = sizeof(float) * 16 * sb::mf::kMaxEntries;
-  if (!attr) {
-    if (cudaFuncSetAttribute(sb::mf::down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)) != cudaSuccess)
-      return SB_ERR_CUDA;
-    attr = true;
-  }
+  int* status = sb::device_status_ptr();
+  if (!status) return SB_ERR_CUDA;
   const int n = T * k;
-  const auto* a = static_cast<__nv_bfloat16*>(act);
-  cudaError_t e = sb::launch_pdl(sb::mf::gate_up_kernel, dim3(2 * sb::sm_count()), dim3(sb::mf::kThreads), 0, st,
-                                 static_cast<const __nv_bfloat16*>(h), h_stride, idx, static_cast<const __nv_bfloat16*>(wgu),
-                                 static_cast<__nv_bfloat16*>(act), n, k, E, H, F);
+  // what a CTA may have (227 KB) less the row lists and the warps' sums
+  const size_t most = 227 * 1024 - sizeof(sb::mf::Ring) - 128;
+  const size_t lists = sb::mf::lists_bytes(n, E), fixed = sb::mf::kRedBytes + lists;
+  const sb::mf::Shape gu = sb::mf::ring_shape(H, most - fixed);
+  if (gu.stages < 2) return SB_ERR_TOO_LARGE;
+  const size_t smem_gu = fixed + static_cast<size_t>(gu.stages) * 16 * gu.piece;
+  // a warp's k steps of a piece: registers for four hold up to 1024 columns
+  cudaError_t e = (gu.piece <= 1024 ? sb::mf::launch_gate_up<4> : sb::mf::launch_gate_up<8>)(h, h_stride, idx, wgu, act, T, k, E, H, F, gu,
+                                                                                              smem_gu, most, status, st);
   if (e != cudaSuccess) return SB_ERR_CUDA;
-  e = sb::launch_pdl(sb::mf::down_kernel, dim3((H + 15) / 16), dim3(sb::mf::kThreads), sizeof(float) * 16 * n, st, a, idx, w,
-                     static_cast<const __nv_bfloat16*>(wd), static_cast<__nv_bfloat16*>(out), T, k, E, H, F);
+  e = sb::mf::launch_down(act, idx, w, wd, out, T, k, E, H, F, sizeof(float) * 16 * static_cast<size_t>(n) + lists, most, st);
   return e == cudaSuccess ? SB_OK : SB_ERR_CUDA;
 }
 

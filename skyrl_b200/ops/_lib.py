@@ -67,20 +67,12 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-class _NoSwitch:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_SWITCH = _NoSwitch()
-
-
-def device_guard(t: torch.Tensor):
-    """Context in which ``t``'s device is the current one, so that a launch and ``stream_ptr`` go to it."""
-    return _NO_SWITCH if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def call_on(dev: int, fn, *args) -> int:
+    """``fn(*args, stream)`` with CUDA device ``dev`` current and on that device's current stream."""
+    if dev == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

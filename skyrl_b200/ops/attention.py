@@ -209,21 +209,22 @@ def paged_layout(block_tables: torch.Tensor, lens: torch.Tensor, block_size: int
     what = "paged_layout"
     if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
         raise ValueError(f"{what}: block tables must be int32 [B, max_blocks] rows, got {block_tables.dtype} {tuple(block_tables.shape)}")
-    B = block_tables.shape[0]
+    B, width = block_tables.shape
+    dev = block_tables.get_device()  # -1 on the CPU
     for t in (lens, starts):
-        if t is not None and (t.shape != (B,) or t.dtype != torch.int32 or not t.is_contiguous() or t.device != block_tables.device):
+        if t is not None and (t.dim() != 1 or t.numel() != B or t.dtype != torch.int32 or not t.is_contiguous() or t.get_device() != dev):
             raise ValueError(f"{what}: lengths must be contiguous int32 [{B}] tensors on the tables' device")
     if not 0 <= total < 2**31 or block_size < 1:
         raise ValueError(f"{what}: total {total} or block size {block_size} is out of range")
-    dev = block_tables.device
-    if dev.type == "cuda":
-        buf = torch.empty(B + 1 + 3 * total, device=dev, dtype=torch.int32)
-        lay = PagedLayout(*buf.split((B + 1, total, total, total)))
-        with _lib.device_guard(buf):
-            code = _k().sb_paged_layout(block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], _lib.ptr(starts),
-                                        lens.data_ptr(), B, block_size, total, *[t.data_ptr() for t in lay], _lib.stream_ptr())
+    if dev >= 0:
+        buf = torch.empty(B + 1 + 3 * total, device=block_tables.device, dtype=torch.int32)
+        at = buf.data_ptr()
+        cu_end, step = at + 4 * (B + 1), 4 * total
+        code = _lib.call_on(dev, _k().sb_paged_layout, block_tables.data_ptr(), block_tables.stride(0), width,
+                            None if starts is None else starts.data_ptr(), lens.data_ptr(), B, block_size, total, at, cu_end,
+                            cu_end + step, cu_end + 2 * step)
         _lib.check(code, "sb_paged_layout")
-        return lay
+        return PagedLayout(*buf.split_with_sizes((B + 1, total, total, total)))
     n = lens.long().clamp_min(0)
     s = torch.zeros_like(n) if starts is None else torch.minimum(starts.long().clamp_min(0), n)
     zero = n.new_zeros(1)

@@ -170,9 +170,9 @@ def build_rope_table(max_pos: int, head_dim: int, theta: float, device, scaling:
     part, ``head_dim`` is the rotated width.  ``scaling``: see ``rope_frequencies``.  Angles are formed in fp64: at
     position 131072 an fp32 angle would already be off by 2^-8."""
     inv, gain = rope_frequencies(head_dim, theta, scaling)
-    ang = torch.arange(max_pos, dtype=torch.float64)[:, None] * inv[None, :]
+    ang = torch.arange(max_pos, dtype=torch.float64, device=device)[:, None] * inv.to(device)[None, :]
     tab = torch.cat([ang.cos(), ang.sin()], dim=-1)
-    return (tab if gain == 1.0 else tab * gain).float().to(device)
+    return (tab if gain == 1.0 else tab * gain).float()
 
 
 def _rope_ref(qkv, pos, table, n_rot_heads, D, sign):

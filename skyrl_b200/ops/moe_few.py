@@ -41,15 +41,17 @@ def _rows(h: torch.Tensor) -> torch.Tensor:
     return h if ok else h.contiguous()
 
 
-def _check_common(what, h, *weights):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (h, *weights)):
+def _check_common(what, h, a, b):
+    if torch.is_grad_enabled() and (h.requires_grad or a.requires_grad or b.requires_grad):
         raise ValueError(f"{what} has no gradient: call it under torch.no_grad() (moe_ffn trains)")
-    if h.dim() != 2 or any(t.dtype != h.dtype or t.device != h.device for t in weights):
+    dt, dev = h.dtype, h.get_device()  # -1 on the CPU
+    if h.dim() != 2 or a.dtype != dt or b.dtype != dt or a.get_device() != dev or b.get_device() != dev:
         raise ValueError(f"{what}: rows [T, H] and weights must have one type and device")
-    if any(not t.is_contiguous() for t in weights):
+    if not a.is_contiguous() or not b.is_contiguous():
         raise ValueError(f"{what}: weights must be contiguous")
-    if h.is_cuda and (h.dtype != torch.bfloat16 or h.shape[1] % 8):
-        raise ValueError(f"{what}: CUDA rows must be bf16 with a width that is a multiple of 8, got {h.dtype} [{h.shape[1]}]")
+    if dev >= 0 and (dt != torch.bfloat16 or h.shape[1] % 8):
+        raise ValueError(f"{what}: CUDA rows must be bf16 with a width that is a multiple of 8, got {dt} [{h.shape[1]}]")
+    return dev
 
 
 def route_few(h: torch.Tensor, router_w: torch.Tensor, top_k: int, norm_topk_prob: bool = True,
@@ -60,16 +62,17 @@ def route_few(h: torch.Tensor, router_w: torch.Tensor, top_k: int, norm_topk_pro
     ``live`` (``[T]`` int32): rows where it is 0 are not routed; they get id -1 and weight 0, so that the expert layer
     reads no weights for them.  A row with a NaN logit gets weights of NaN and valid ids."""
     what = "route_few"
-    _check_common(what, h, router_w)
+    dev = _check_common(what, h, router_w, router_w)
     T, H = h.shape
     if router_w.dim() != 2 or router_w.shape[1] != H:
         raise ValueError(f"{what}: router weights {tuple(router_w.shape)} do not fit rows of width {H}")
     E = router_w.shape[0]
     if not 1 <= top_k <= min(MAX_TOP_K, E) or E > MAX_EXPERTS:
         raise ValueError(f"{what}: top {top_k} of {E} experts is out of range (at most {MAX_TOP_K} of {MAX_EXPERTS})")
-    if live is not None and (live.shape != (T,) or live.dtype != torch.int32 or live.device != h.device or not live.is_contiguous()):
+    if live is not None and (live.dim() != 1 or live.numel() != T or live.dtype != torch.int32 or live.get_device() != dev
+                             or not live.is_contiguous()):
         raise ValueError(f"{what}: live must be a contiguous int32 [{T}] tensor on the rows' device")
-    if not h.is_cuda:
+    if dev < 0:
         z = h.double() @ router_w.double().t()
         bad = torch.isnan(z).any(-1)
         z = torch.where(torch.isnan(z), torch.full_like(z, float("-inf")), z)
@@ -87,9 +90,9 @@ def route_few(h: torch.Tensor, router_w: torch.Tensor, top_k: int, norm_topk_pro
     if T == 0:
         return w, idx
     h = _rows(h)
-    with _lib.device_guard(h):
-        code = _k().sb_moe_few_route(h.data_ptr(), h.stride(0), router_w.data_ptr(), _lib.ptr(live), w.data_ptr(), idx.data_ptr(),
-                                     T, E, H, top_k, int(norm_topk_prob), _lib.stream_ptr())
+    code = _lib.call_on(dev, _k().sb_moe_few_route, h.data_ptr(), h.stride(0), router_w.data_ptr(),
+                        None if live is None else live.data_ptr(), w.data_ptr(), idx.data_ptr(), T, E, H, top_k,
+                        bool(norm_topk_prob))
     _lib.check(code, "sb_moe_few_route")
     return w, idx
 
@@ -100,19 +103,19 @@ def expert_ffn_few(h: torch.Tensor, w: torch.Tensor, idx: torch.Tensor, wgu: tor
     ``[E, H, F]``; at most 2048 ``(t, s)`` pairs.  A slot whose id lies outside ``[0, E)`` contributes nothing (a row
     without valid slots is zero); an expert may appear in several slots of a row."""
     what = "expert_ffn_few"
-    _check_common(what, h, wgu, wd)
+    dev = _check_common(what, h, wgu, wd)
     T, H = h.shape
     if wgu.dim() != 3 or wd.dim() != 3 or wgu.shape[1] != 2 * wd.shape[2] or wgu.shape[2] != H or wd.shape[:2] != (wgu.shape[0], H):
         raise ValueError(f"{what}: weights {tuple(wgu.shape)}, {tuple(wd.shape)} do not fit rows of width {H}")
     E, F = wgu.shape[0], wd.shape[2]
     if idx.dim() != 2 or idx.shape[0] != T or w.shape != idx.shape or idx.dtype != torch.int32 or w.dtype != torch.float32:
         raise ValueError(f"{what}: weights and ids must be fp32 and int32 [{T}, k] tensors")
-    if not idx.is_contiguous() or not w.is_contiguous() or idx.device != h.device or w.device != h.device:
+    if not idx.is_contiguous() or not w.is_contiguous() or idx.get_device() != dev or w.get_device() != dev:
         raise ValueError(f"{what}: weights and ids must be contiguous and on the rows' device")
     k = idx.shape[1]
     if k < 1 or T * k > MAX_ENTRIES or E > MAX_EXPERTS or F < 1:
         raise ValueError(f"{what}: {T} x {k} entries over {E} experts are out of range (at most {MAX_ENTRIES} over {MAX_EXPERTS})")
-    if not h.is_cuda:
+    if dev < 0:
         out = torch.zeros(T, H, dtype=torch.float32)
         y = torch.zeros(T * k, H, dtype=torch.float32)
         flat = idx.reshape(-1).long()
@@ -128,13 +131,12 @@ def expert_ffn_few(h: torch.Tensor, w: torch.Tensor, idx: torch.Tensor, wgu: tor
         return out.add_(terms.sum(1)).to(h.dtype)
     if F % 8:
         raise ValueError(f"{what}: the experts' width must be a multiple of 8 on CUDA, got {F}")
-    out = torch.empty((T, H), device=h.device, dtype=h.dtype)
+    out = torch.empty_like(h, memory_format=torch.contiguous_format)
     if T == 0:
         return out
     h = _rows(h)
-    act = torch.empty((T * k, F), device=h.device, dtype=h.dtype)
-    with _lib.device_guard(h):
-        code = _k().sb_moe_few_experts(h.data_ptr(), h.stride(0), w.data_ptr(), idx.data_ptr(), wgu.data_ptr(), wd.data_ptr(),
-                                       act.data_ptr(), out.data_ptr(), T, k, E, H, F, _lib.stream_ptr())
+    act = h.new_empty(T * k * F)
+    code = _lib.call_on(dev, _k().sb_moe_few_experts, h.data_ptr(), h.stride(0), w.data_ptr(), idx.data_ptr(), wgu.data_ptr(),
+                        wd.data_ptr(), act.data_ptr(), out.data_ptr(), T, k, E, H, F)
     _lib.check(code, "sb_moe_few_experts")
     return out

@@ -38,26 +38,26 @@ def _k():
 
 # ----------------------------------------------------------------------------- checks
 def _check(rows, pos, table, nq, nk, head_dim, q_norm, k_norm, what):
-    T, W = rows.shape[-2], rows.shape[-1]
-    if nq < 0 or nk < 0 or nq + nk < 1 or head_dim < 1 or W % head_dim or W // head_dim < nq + nk:
+    T, W = rows.shape[-2:]
+    if nq < 0 or nk < 0 or nq + nk < 1 or head_dim < 1 or W % head_dim or W < (nq + nk) * head_dim:
         raise ValueError(f"{what}: rows of width {W} do not hold {nq} + {nk} rotated heads of size {head_dim}")
     if head_dim > _MAX_HEAD_DIM:
         raise ValueError(f"{what}: head size {head_dim} is above {_MAX_HEAD_DIM}")
     if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
         raise ValueError(f"{what}: the rope table must be a contiguous fp32 [positions, rotated width] tensor")
-    R = table.shape[1]
-    if R < 2 or R % 2 or R > head_dim or table.shape[0] < 1:
+    n_pos, R = table.shape
+    if R < 2 or R % 2 or R > head_dim or n_pos < 1:
         raise ValueError(f"{what}: rope table {tuple(table.shape)} does not fit heads of size {head_dim}")
-    if pos.dtype != torch.int32 or pos.dim() != 1 or pos.shape[0] != T or not pos.is_contiguous():
+    if pos.dtype != torch.int32 or pos.dim() != 1 or pos.numel() != T or not pos.is_contiguous():
         raise ValueError(f"{what}: positions must be a contiguous int32 [{T}] tensor, got {pos.dtype} {tuple(pos.shape)}")
+    dev = rows.get_device()  # -1 on the CPU
+    if pos.get_device() != dev or table.get_device() != dev:
+        raise ValueError(f"{what}: rows, positions and table must be on one device")
     if (q_norm is None) != (k_norm is None):
         raise ValueError(f"{what}: q_norm and k_norm go together")
-    dev = rows.device
-    if pos.device != dev or table.device != dev:
-        raise ValueError(f"{what}: rows, positions and table must be on one device")
     if q_norm is not None:
         for w in (q_norm, k_norm):
-            if w.shape != (head_dim,) or not w.is_contiguous() or w.device != dev:
+            if w.dim() != 1 or w.numel() != head_dim or not w.is_contiguous() or w.get_device() != dev:
                 raise ValueError(f"{what}: norm weights must be contiguous [{head_dim}] tensors on the rows' device")
 
 
@@ -128,27 +128,31 @@ def _launch_fwd(src, dst, q_norm, k_norm, pos, table, nq, nk, D, eps, interleave
     T, W = dst.shape
     if T == 0:
         return dst
-    with _lib.device_guard(dst):
-        code = _k().sb_qk_rope_fwd(
-            src.data_ptr(), dst.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), pos.data_ptr(), table.data_ptr(),
-            _lib.ptr(slots), _lib.ptr(k_cache), _lib.ptr(v_cache),
-            0 if k_cache is None else k_cache.shape[0] * k_cache.shape[1], src.stride(-2), dst.stride(0),
-            src.stride(0) if n_part else 0, n_part, table.shape[0], T, nq, nk, W // D, D, table.shape[1],
-            _DTYPE[dst.dtype], int(interleaved), eps, sign, _lib.stream_ptr())
+    max_pos, R = table.shape
+    code = _lib.call_on(
+        dst.get_device(), _k().sb_qk_rope_fwd, src.data_ptr(), dst.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
+        None if k_norm is None else k_norm.data_ptr(), pos.data_ptr(), table.data_ptr(),
+        None if slots is None else slots.data_ptr(), None if k_cache is None else k_cache.data_ptr(),
+        None if v_cache is None else v_cache.data_ptr(), 0 if k_cache is None else k_cache.shape[0] * k_cache.shape[1],
+        src.stride(-2), dst.stride(0), src.stride(0) if n_part else 0, n_part, max_pos, T, nq, nk, W // D, D, R,
+        _DTYPE[dst.dtype], interleaved, eps, sign)
     _lib.check(code, "sb_qk_rope_fwd")
     return dst
 
 
+def _rows_like(x):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 class _QKNormRopeFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved):
-        ctx.meta = (nq, nk, D, eps, interleaved)
+    def forward(ctx, x, q_norm, k_norm, pos, table, meta):
+        ctx.meta = meta
         if x.is_cuda:
             x = _row_major(x)
-            out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-            _launch_fwd(x, out, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, 1.0)
+            out = _launch_fwd(x, _rows_like(x), q_norm, k_norm, pos, table, *meta, 1.0)
         else:
-            out = _fwd_ref(x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, 1.0)
+            out = _fwd_ref(x, q_norm, k_norm, pos, table, *meta, 1.0)
         if q_norm is None:
             ctx.save_for_backward(pos, table)
         else:
@@ -158,25 +162,23 @@ class _QKNormRopeFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        nq, nk, D, eps, interleaved = ctx.meta
-        none = (None,) * 7
+        if torch.is_grad_enabled():
+            raise RuntimeError("rotary / qk_norm_rope have no second derivative")
         pos, table, *rest = ctx.saved_tensors
         if not rest:
             if not dy.is_cuda:
-                return _fwd_ref(dy, None, None, pos, table, nq, nk, D, eps, interleaved, -1.0), None, None, *none
+                return _fwd_ref(dy, None, None, pos, table, *ctx.meta, -1.0), None, None, None, None, None
             dy = _row_major(dy)
-            dx = torch.empty(dy.shape, device=dy.device, dtype=dy.dtype)
-            return _launch_fwd(dy, dx, None, None, pos, table, nq, nk, D, eps, interleaved, -1.0), None, None, *none
+            return _launch_fwd(dy, _rows_like(dy), None, None, pos, table, *ctx.meta, -1.0), None, None, None, None, None
         x, q_norm, k_norm = rest
-        want = ctx.needs_input_grad[1:3]
-        if not dy.is_cuda:
-            dx, *dws = _bwd_ref(dy, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved)
+        want, main_grads = ctx.needs_input_grad[1:3], ctx.main_grads
+        if dy.is_cuda:
+            dx, *dws = _launch_bwd(dy, x, q_norm, k_norm, pos, table, *ctx.meta, want, main_grads)
         else:
-            dx, *dws = _launch_bwd(dy, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, want, ctx.main_grads)
+            dx, *dws = _bwd_ref(dy, x, q_norm, k_norm, pos, table, *ctx.meta)
         out = []
-        for dw, w, mg, on in zip(dws, (q_norm, k_norm), ctx.main_grads, want):
+        for dw, w, mg, on in zip(dws, (q_norm, k_norm), main_grads, want):
             if not on or dw is None:
                 out.append(None)
             elif mg is not None:
@@ -184,34 +186,35 @@ class _QKNormRopeFn(torch.autograd.Function):
                 out.append(None)
             else:
                 out.append(dw.to(w.dtype))
-        return dx, *out, *none
+        return dx, *out, None, None, None
 
 
 def _launch_bwd(dy, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, want, main_grads):
     """Returns ``(dx, dqw, dkw)``; a weight gradient that the kernel added to its fp32 ``main_grad`` is None."""
     dy = _row_major(dy)
     T, W = x.shape
-    dx = torch.empty((T, W), device=x.device, dtype=x.dtype)
+    dx = _rows_like(x)
     wanted = [(g, w) for g, w, on in zip(main_grads, (q_norm, k_norm), want) if on]
     # added in place where every wanted gradient has its fp32 buffer, stored in the weights' type where none has; a mix
     # goes through fp32 zeros
     direct = bool(wanted) and all(g is not None and g.is_contiguous() and g.dtype == torch.float32 for g, _ in wanted)
     mixed = not direct and any(g is not None for g, _ in wanted)
-    dws = [None if not on else g if direct else torch.zeros_like(w, dtype=torch.float32) if mixed else torch.empty_like(w)
-           for g, w, on in zip(main_grads, (q_norm, k_norm), want)]
+    dqw, dkw = [None if not on else g if direct else torch.zeros_like(w, dtype=torch.float32) if mixed else torch.empty_like(w)
+                for g, w, on in zip(main_grads, (q_norm, k_norm), want)]
     if T == 0:
-        return (dx, *(None if direct or g is None else g.zero_() for g in dws))
+        return (dx, *(None if direct or g is None else g.zero_() for g in (dqw, dkw)))
     lib = _k()
-    n_parts = lib.sb_qk_norm_rope_bwd_parts(T, W // D, D)
+    max_pos, R = table.shape
+    heads = W // D
+    n_parts = lib.sb_qk_norm_rope_bwd_parts(T, heads, D)
     part = torch.empty(n_parts * 2 * D, device=x.device, dtype=torch.float32) if wanted else None
-    with _lib.device_guard(x):
-        code = lib.sb_qk_norm_rope_bwd(
-            dy.data_ptr(), x.data_ptr(), dx.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), pos.data_ptr(),
-            table.data_ptr(), _lib.ptr(dws[0]), _lib.ptr(dws[1]), _lib.ptr(part), n_parts, dy.stride(0), x.stride(0),
-            dx.stride(0), table.shape[0], T, nq, nk, W // D, D, table.shape[1], _DTYPE[x.dtype], int(interleaved),
-            int(direct or mixed), eps, _lib.stream_ptr())
+    code = _lib.call_on(
+        x.get_device(), lib.sb_qk_norm_rope_bwd, dy.data_ptr(), x.data_ptr(), dx.data_ptr(), q_norm.data_ptr(),
+        k_norm.data_ptr(), pos.data_ptr(), table.data_ptr(), None if dqw is None else dqw.data_ptr(),
+        None if dkw is None else dkw.data_ptr(), None if part is None else part.data_ptr(), n_parts, dy.stride(0), x.stride(0),
+        dx.stride(0), max_pos, T, nq, nk, heads, D, R, _DTYPE[x.dtype], interleaved, direct or mixed, eps)
     _lib.check(code, "sb_qk_norm_rope_bwd")
-    return (dx, None, None) if direct else (dx, *dws)
+    return (dx, None, None) if direct else (dx, dqw, dkw)
 
 
 # ----------------------------------------------------------------------------- entry points
@@ -221,7 +224,7 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, n_rot_heads:
     copied.  Returns new rows (``elementwise.rope`` is the in-place form for whole heads in the half layout)."""
     _check_rows(x, "rotary")
     _check(x, pos, table, n_rot_heads, 0, head_dim, None, None, "rotary")
-    return _QKNormRopeFn.apply(x, None, None, pos, table, n_rot_heads, 0, head_dim, 0.0, bool(interleaved))
+    return _QKNormRopeFn.apply(x, None, None, pos, table, (n_rot_heads, 0, head_dim, 0.0, bool(interleaved)))
 
 
 def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, pos: torch.Tensor, table: torch.Tensor,
@@ -235,7 +238,7 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, 
     _check(qkv, pos, table, nq, nkv, head_dim, q_norm, k_norm, "qk_norm_rope")
     if q_norm.dtype != qkv.dtype or k_norm.dtype != qkv.dtype:
         raise ValueError("qk_norm_rope: norm weights must have the rows' type")
-    return _QKNormRopeFn.apply(qkv, q_norm, k_norm, pos, table, nq, nkv, head_dim, float(eps), bool(interleaved))
+    return _QKNormRopeFn.apply(qkv, q_norm, k_norm, pos, table, (nq, nkv, head_dim, float(eps), bool(interleaved)))
 
 
 def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -270,11 +273,11 @@ def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cac
         raise ValueError(f"{what}: caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} do not hold {nkv} heads of size {head_dim}")
     if not k_cache.is_contiguous() or not v_cache.is_contiguous() or k_cache.dim() != 4:
         raise ValueError(f"{what}: caches must be contiguous [blocks, block_size, heads, head_dim] tensors")
-    if slots.dtype != torch.int32 or slots.shape != (T,) or not slots.is_contiguous():
+    if slots.dtype != torch.int32 or slots.dim() != 1 or slots.numel() != T or not slots.is_contiguous():
         raise ValueError(f"{what}: slots must be a contiguous int32 [{T}] tensor")
-    if not (k_cache.device == v_cache.device == slots.device == x.device):
+    if not (k_cache.get_device() == v_cache.get_device() == slots.get_device() == x.get_device()):
         raise ValueError(f"{what}: rows, slots and caches must be on one device")
-    if out is not None and (out.shape != (T, W) or out.dtype != dt or out.device != x.device or out.stride(1) != 1
+    if out is not None and (out.shape != (T, W) or out.dtype != dt or out.get_device() != x.get_device() or out.stride(1) != 1
                             or (T > 1 and out.stride(0) < W)):
         raise ValueError(f"{what}: out must be [{T}, {W}] rows in the caches' type")
     if not x.is_cuda:
