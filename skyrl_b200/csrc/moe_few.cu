@@ -23,157 +23,159 @@ namespace mf {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxEntries = 2048;
 constexpr int kMaxTopK = 16;
 
-// ---------------------------------------------------------------------------
-// Router.  A cluster of eight CTAs takes kTok tokens and an eighth of the experts each; the logits of token i meet in
-// CTA i's shared memory.  Products of bf16 are exact in fp32; eight of them are summed there and the rest in fp64, so
-// that experts whose logits lie next to one another are ordered by the values and not by the order of the sum.
-// ---------------------------------------------------------------------------
-constexpr int kCluster = 8;
-
-__device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
-  const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&a);
-  const __nv_bfloat162* y = reinterpret_cast<const __nv_bfloat162*>(&b);
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = __bfloat1622float2(x[i]), q = __bfloat1622float2(y[i]);
-    s = fmaf(p.x, q.x, s);
-    s = fmaf(p.y, q.y, s);
-  }
-  return s;
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int kTok>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
+// ---------------------------------------------------------------------------
+// Router.  A cluster of eight CTAs takes eight tokens and an eighth of the experts each, 16 experts at a time; the CTA's
+// warps split the columns, and the logits of token i meet in CTA i's shared memory.  Products of bf16 are exact in the
+// matrix unit; its fp32 sums are taken out every 32 columns and carried on in two fp32 words, so that experts whose
+// logits lie next to one another are ordered by the values and not by the rounding of a long sum.
+// The k largest are found by rank, the number of experts that come before one: all are compared with one another at once,
+// where k rounds of a maximum would wait for one another.  Beyond kRankGroup experts, passes over groups leave k
+// candidates each, and a last pass ranks those.
+// ---------------------------------------------------------------------------
+constexpr int kCluster = 8;  // CTAs, and tokens
+constexpr int kRouteThreads = 256;
+constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kRankGroup = 128;  // entries ranked in a pass, two lanes each
+
+// Order-preserving key of a logit, unique: the lowest ten bits hold the expert, the lower one first among equals.  A NaN
+// comes last.
+__device__ __forceinline__ unsigned long long logit_key(double v, int e) {
+  const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
+  const unsigned long long k = v != v ? 0ull : (b >> 63 ? ~b : b | 0x8000000000000000ull);
+  return (k & ~1023ull) | static_cast<unsigned long long>(1023 - e);
+}
+__device__ __forceinline__ int key_expert(unsigned long long k) { return 1023 - static_cast<int>(k & 1023); }
+
+// Entries of key[0..n) above `mine`, counted by two neighbouring lanes.
+__device__ __forceinline__ int rank_of(const unsigned long long* key, int n, unsigned long long mine) {
+  int before = 0;
+#pragma unroll 8
+  for (int j = threadIdx.x & 1; j < n; j += 2) before += key[j] > mine;
+  return before + __shfl_xor_sync(0xffffffffu, before, 1);
+}
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kRouteThreads, 2)
 route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv_bfloat16* __restrict__ rw,
              const int* __restrict__ live, float* __restrict__ w, int* __restrict__ idx, int T, int E, int H, int k, int norm) {
+  __shared__ float2 part[kRouteWarps][4][32];
+  __shared__ unsigned long long key[kMaxExperts], cand[kRankGroup];
+  __shared__ int n_cand, chosen[kMaxTopK];
   extern __shared__ double logits[];  // [E], of token t0 + rank
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = static_cast<int>(blockIdx.x / kCluster) * kTok;
+  const int t0 = static_cast<int>(blockIdx.x / kCluster) * kCluster;
   cluster.barrier_arrive();
-  bool waited = false;
+  if (threadIdx.x == 0) n_cand = 0;
   const int per = (E + kCluster - 1) / kCluster;
   const int e_hi = min(E, (rank + 1) * per);
-  const int nv = H >> 3;
-  for (int e = rank * per + warp; e < e_hi; e += 2 * kWarps) {  // two experts at a time: their rows are all under way at once
-    const bool two = e + kWarps < e_hi;
-    const uint4* r0 = reinterpret_cast<const uint4*>(rw + static_cast<size_t>(e) * H);
-    const uint4* r1 = reinterpret_cast<const uint4*>(rw + static_cast<size_t>(two ? e + kWarps : e) * H);
-    double acc[2][kTok];
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) acc[0][i] = acc[1][i] = 0.0;
-    constexpr int kUnroll = kTok == 1 ? 8 : 4;
-    for (int v0 = lane; v0 < nv; v0 += 32 * kUnroll) {
-      uint4 a[kUnroll], b[kUnroll];
+  const int g = lane >> 2, t4 = lane & 3;
+  const int steps = (H + 31) >> 5, s0 = warp * steps / kRouteWarps, s1 = (warp + 1) * steps / kRouteWarps;
+  const __nv_bfloat16* x = h + static_cast<size_t>(min(t0 + g, T - 1)) * h_stride + 8 * t4;  // rows behind the last: not used
+  bool waited = false;
+  for (int e0 = rank * per; e0 < e_hi; e0 += 16) {
+    const __nv_bfloat16* top = rw + static_cast<size_t>(min(e0 + g, e_hi - 1)) * H + 8 * t4;
+    const __nv_bfloat16* low = rw + static_cast<size_t>(min(e0 + g + 8, e_hi - 1)) * H + 8 * t4;
+    float hi[4] = {0.f, 0.f, 0.f, 0.f}, lo[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kUnroll = 4;
+    for (int s = s0; s < s1; s += kUnroll) {
+      uint4 a[kUnroll], b[kUnroll], v[kUnroll];
 #pragma unroll
       for (int j = 0; j < kUnroll; ++j) {
-        const int v = v0 + 32 * j;
-        a[j] = v < nv ? __ldg(r0 + v) : make_uint4(0, 0, 0, 0);
-        b[j] = v < nv ? __ldg(r1 + v) : make_uint4(0, 0, 0, 0);
+        const int col = (s + j) * 32;
+        const bool ok = s + j < s1 && col + 8 * t4 < H;
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        a[j] = ok ? __ldg(reinterpret_cast<const uint4*>(top + col)) : z;
+        b[j] = ok ? __ldg(reinterpret_cast<const uint4*>(low + col)) : z;
+        v[j] = ok ? __ldg(reinterpret_cast<const uint4*>(x + col)) : z;
       }
 #pragma unroll
       for (int j = 0; j < kUnroll; ++j) {
-        const int v = v0 + 32 * j;
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_bf16(d, a[j].x, b[j].x, a[j].y, b[j].y, v[j].x, v[j].y);
+        mma_bf16(d, a[j].z, b[j].z, a[j].w, b[j].w, v[j].z, v[j].w);
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) {
-          if (v >= nv || t0 + i >= T) continue;
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(h + static_cast<size_t>(t0 + i) * h_stride) + v);
-          acc[0][i] += static_cast<double>(dot8(a[j], x));
-          acc[1][i] += static_cast<double>(dot8(b[j], x));
+        for (int c = 0; c < 4; ++c) {
+          const float sum = hi[c] + d[c], back = sum - hi[c];
+          lo[c] += (hi[c] - (sum - back)) + (d[c] - back);  // what the addition rounded away
+          hi[c] = sum;
         }
       }
     }
+    if (waited) __syncthreads();  // the sums of the 16 experts before have been read
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-      for (int i = 0; i < kTok; ++i) {
-        acc[0][i] += __shfl_xor_sync(0xffffffffu, acc[0][i], o);
-        acc[1][i] += __shfl_xor_sync(0xffffffffu, acc[1][i], o);
-      }
+    for (int c = 0; c < 4; ++c) part[warp][c][lane] = make_float2(hi[c], lo[c]);
+    __syncthreads();
     if (!waited) cluster.barrier_wait();  // every CTA of the cluster runs before its shared memory is written
     waited = true;
-    if (lane == 0) {
+    if (threadIdx.x < 128) {
+      const int c = threadIdx.x >> 5;  // fragment component: expert g + 8 (c / 2), token 2 t4 + c % 2
+      double v = 0.0;
 #pragma unroll
-      for (int i = 0; i < kTok; ++i) {
-        double* dst = cluster.map_shared_rank(logits, i);
-        dst[e] = acc[0][i] + 0.0;  // -0 counts as +0
-        if (two) dst[e + kWarps] = acc[1][i] + 0.0;
-      }
+      for (int i = 0; i < kRouteWarps; ++i) v += static_cast<double>(part[i][c][lane].x) + static_cast<double>(part[i][c][lane].y);
+      const int e = e0 + g + 8 * (c >> 1);
+      if (e < e_hi) cluster.map_shared_rank(logits, 2 * t4 + (c & 1))[e] = v + 0.0;  // -0 counts as +0
     }
   }
   if (!waited) cluster.barrier_wait();
   cluster.sync();
   const int t = t0 + rank;
-  if (rank >= kTok || t >= T || warp != 0) return;
+  if (t >= T) return;
   if (live && live[t] == 0) {
-    if (lane < k) {
-      w[static_cast<size_t>(t) * k + lane] = 0.f;
-      idx[static_cast<size_t>(t) * k + lane] = -1;
+    if (threadIdx.x < k) {
+      w[static_cast<size_t>(t) * k + threadIdx.x] = 0.f;
+      idx[static_cast<size_t>(t) * k + threadIdx.x] = -1;
     }
     return;
   }
-  // k rounds of a warp-wide maximum over order-preserving 64-bit keys, the high words first.  A lane keeps the best of
-  // its experts lane + 32 j and looks again only after it has lost it.  Ties go to the lower expert.  A NaN counts as
-  // the smallest value, so that the indices stay in range, and makes the row's weights NaN.
-  uint32_t taken = 0;  // bit j: expert lane + 32 j
-  bool bad = false;
-  unsigned long long best = 0;
-  int best_e = 0x7fffffff;
-  auto look = [&]() {
-    best = 0;
-    best_e = 0x7fffffff;
-    for (int j = 0, e = lane; e < E; ++j, e += 32) {
-      const double v = logits[e];
-      const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
-      const bool nan = v != v;
-      bad |= nan;
-      const unsigned long long key = nan ? 0ull : (b >> 63 ? ~b : b | 0x8000000000000000ull);
-      if (!(taken >> j & 1) && (best_e == 0x7fffffff || key > best)) {
-        best = key;
-        best_e = e;
-      }
-    }
-  };
-  look();
-  double top = 0.0;
-  float mine = 0.f, sel = 0.f;
-  int my_e = 0;
-  for (int s = 0; s < k; ++s) {
-    const bool have = best_e != 0x7fffffff;
-    const uint32_t hi = have ? static_cast<uint32_t>(best >> 32) : 0u, lo = have ? static_cast<uint32_t>(best) : 0u;
-    const uint32_t top_hi = __reduce_max_sync(0xffffffffu, hi);
-    const uint32_t top_lo = __reduce_max_sync(0xffffffffu, hi == top_hi ? lo : 0u);
-    const uint32_t win = __reduce_min_sync(0xffffffffu, have && hi == top_hi && lo == top_lo ? static_cast<uint32_t>(best_e) : 0x7fffffffu);
-    if (have && best_e == static_cast<int>(win)) {
-      taken |= 1u << (win >> 5);
-      look();
-    }
-    const double v = logits[win];
-    if (s == 0) top = v;
-    const float p = expf(static_cast<float>(v - top));
-    sel += p;
-    if (lane == s) {
-      mine = p;
-      my_e = static_cast<int>(win);
-    }
+  int bad = 0;
+  for (int e = threadIdx.x; e < E; e += kRouteThreads) {
+    const double v = logits[e];
+    bad |= v != v;
+    key[e] = logit_key(v, e);
   }
-  float all = sel;
-  if (!norm) {
-    all = 0.f;
+  bad = __syncthreads_or(bad);
+  const int slot = threadIdx.x >> 1;
+  const unsigned long long* of = key;
+  int n = E;
+  if (E > kRankGroup) {  // at most eight groups, with k <= 16 candidates each
+    for (int g0 = 0; g0 < E; g0 += kRankGroup) {
+      const int gn = min(kRankGroup, E - g0);
+      const unsigned long long mine = key[g0 + min(slot, gn - 1)];
+      const int before = rank_of(key + g0, gn, mine);
+      if (slot < gn && !(threadIdx.x & 1) && before < k) cand[atomicAdd(&n_cand, 1)] = mine;
+    }
+    __syncthreads();
+    n = n_cand;
+    of = cand;
+  }
+  const unsigned long long mine = of[min(slot, n - 1)];
+  const int before = rank_of(of, n, mine);
+  if (slot < n && !(threadIdx.x & 1) && before < k) chosen[before] = key_expert(mine);
+  __syncthreads();
+  if (warp != 0) return;
+  const int my_e = lane < k ? chosen[lane] : chosen[0];
+  const double top = logits[chosen[0]];
+  const float p = expf(static_cast<float>(logits[my_e] - top));
+  float all = 0.f;
+  if (norm)
+    all = lane < k ? p : 0.f;
+  else
     for (int e = lane; e < E; e += 32) all += expf(static_cast<float>(logits[e] - top));
-    all = warp_sum(all);
-  }
-  bad = __any_sync(0xffffffffu, bad);
+  all = warp_sum(all);
   if (lane < k) {
-    w[static_cast<size_t>(t) * k + lane] = bad ? __int_as_float(0x7fffffff) : mine / all;
+    w[static_cast<size_t>(t) * k + lane] = bad ? __int_as_float(0x7fffffff) : p / all;
     idx[static_cast<size_t>(t) * k + lane] = my_e;
   }
 }
@@ -191,20 +193,23 @@ struct Lists {
   unsigned short* used;     // [E] experts that have entries, ascending
   unsigned short* unit0;    // [E + 1] first unit of the i-th used expert
   unsigned short* entry;    // [n]
-  int* count;               // used experts, units, rows of the largest unit
+  int* count;               // per 32 experts: rows | units << 16, used experts, rows of the largest expert
   int n_used, n_units, most;
 };
 
-__host__ __device__ constexpr int lists_bytes(int n, int E) { return (4 * E + 2 * (E + 1) * 2 + 2 * E + 2 * n + 16 + 127) / 128 * 128; }
+__host__ __device__ constexpr int lists_bytes(int n, int E) { 
+  return (4 * 3 * 32 + 4 * E + 2 * (E + 1) * 2 + 2 * E + 2 * n + 127) / 128 * 128;
+ }
 
 __device__ __forceinline__ Lists build_lists(char* smem, const int* __restrict__ idx, int n, int E) {
   Lists L;
   L.count = reinterpret_cast<int*>(smem);
-  L.cursor = L.count + 4;
+  L.cursor = L.count + 3 * 32;
   L.first = reinterpret_cast<unsigned short*>(L.cursor + E);
   L.unit0 = L.first + E + 1;
   L.used = L.unit0 + E + 1;
   L.entry = L.used + E;
+  const int lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < E; e += blockDim.x) L.cursor[e] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
@@ -212,56 +217,62 @@ __device__ __forceinline__ Lists build_lists(char* smem, const int* __restrict__
     if (e >= 0 && e < E) atomicAdd(&L.cursor[e], 1);
   }
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    int run = 0, used = 0, units = 0, most = 0;
-    for (int base = 0; base < E; base += 32) {
-      const int e = base + lane;
-      const int c = e < E ? L.cursor[e] : 0;
-      // rows in the low half, units in the high half: neither passes 16 bits (at most kMaxEntries of each)
-      int inc = c | ((c + kUnitRows - 1) / kUnitRows) << 16;
-      const int own = inc;
-      most = max(most, c);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      const unsigned int has = __ballot_sync(0xffffffffu, c > 0);
-      if (e < E) {
-        L.cursor[e] = run + ((inc - own) & 0xffff);
-        L.first[e] = static_cast<unsigned short>(L.cursor[e]);
-        if (c > 0) {
-          const int a = used + __popc(has & ((1u << lane) - 1u));
-          L.used[a] = static_cast<unsigned short>(e);
-          L.unit0[a] = static_cast<unsigned short>(units + ((inc - own) >> 16));
-        }
-      }
-      const int tot = __shfl_sync(0xffffffffu, inc, 31);
-      run += tot & 0xffff;
-      units += tot >> 16;
-      used += __popc(has);
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
+  // a warp takes 32 experts at a time: totals first, then offsets from the totals before.  Rows in the low half, units in
+  // the high half: neither passes 16 bits (at most kMaxEntries of each).
+  const int chunks = (E + 31) >> 5, warps = blockDim.x >> 5;
+  for (int c = threadIdx.x >> 5; c < chunks; c += warps) {
+    const int e = c * 32 + lane;
+    const int rows = e < E ? L.cursor[e] : 0;
+    const int sum = __reduce_add_sync(0xffffffffu, rows | ((rows + kUnitRows - 1) / kUnitRows) << 16);
+    const int most = __reduce_max_sync(0xffffffffu, rows);
+    const unsigned int has = __ballot_sync(0xffffffffu, rows > 0);
     if (lane == 0) {
-      L.first[E] = static_cast<unsigned short>(run);
-      L.unit0[used] = static_cast<unsigned short>(units);
-      L.count[0] = used;
-      L.count[1] = units;
-      L.count[2] = min(most, kUnitRows);
+      L.count[c] = sum;
+      L.count[32 + c] = __popc(has);
+      L.count[64 + c] = most;
     }
   }
   __syncthreads();
-  L.n_used = L.count[0];
-  L.n_units = L.count[1];
-  L.most = L.count[2];
+  {
+    const bool on = lane < chunks;
+    const int sum = __reduce_add_sync(0xffffffffu, on ? L.count[lane] : 0);
+    L.n_units = sum >> 16;
+    L.n_used = __reduce_add_sync(0xffffffffu, on ? L.count[32 + lane] : 0);
+    L.most = min(kUnitRows, __reduce_max_sync(0xffffffffu, on ? L.count[64 + lane] : 0));
+    if (threadIdx.x == 0) {
+      L.first[E] = static_cast<unsigned short>(sum & 0xffff);
+      L.unit0[L.n_used] = static_cast<unsigned short>(sum >> 16);
+    }
+  }
+  for (int c = threadIdx.x >> 5; c < chunks; c += warps) {
+    const int e = c * 32 + lane;
+    const int rows = e < E ? L.cursor[e] : 0;
+    const int own = rows | ((rows + kUnitRows - 1) / kUnitRows) << 16;
+    int inc = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const int at = __reduce_add_sync(0xffffffffu, lane < c ? L.count[lane] : 0) + inc - own;
+    const int a = __reduce_add_sync(0xffffffffu, lane < c ? L.count[32 + lane] : 0) +
+                  __popc(__ballot_sync(0xffffffffu, rows > 0) & ((1u << lane) - 1u));
+    if (e < E) {
+      L.cursor[e] = at & 0xffff;
+      L.first[e] = static_cast<unsigned short>(at & 0xffff);
+      if (rows > 0) {
+        L.used[a] = static_cast<unsigned short>(e);
+        L.unit0[a] = static_cast<unsigned short>(at >> 16);
+      }
+    }
+  }
+  __syncthreads();
   if (L.n_units == L.n_used) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
       const int e = idx[i];
       if (e >= 0 && e < E) L.entry[atomicAdd(&L.cursor[e], 1)] = static_cast<unsigned short>(i);
     }
   } else if (threadIdx.x < 32) {  // in the entries' order, 32 at a time
-    const int lane = threadIdx.x;
     for (int base = 0; base < n; base += 32) {
       const int i = base + lane;
       int e = i < n ? idx[i] : -1;
@@ -296,13 +307,6 @@ __device__ __forceinline__ Unit unit_at(const Lists& L, int unit) {
   u.r0 = L.first[u.e] + (unit - L.unit0[lo]) * kUnitRows;
   u.r1 = min(static_cast<int>(L.first[u.e + 1]), u.r0 + kUnitRows);
   return u;
-}
-
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // ---------------------------------------------------------------------------
@@ -701,15 +705,9 @@ int sb_moe_few_route(const void* h, long long h_stride, const void* router, cons
   if (T <= 0 || E <= 0 || E > sb::mf::kMaxExperts || H <= 0 || (H & 7) || k <= 0 || k > sb::mf::kMaxTopK || k > E || (h_stride & 7))
     return SB_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(router)) & 15) return SB_ERR_ARG;
-  const size_t smem = sizeof(double) * E;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const auto* hp = static_cast<const __nv_bfloat16*>(h);
-  const auto* rp = static_cast<const __nv_bfloat16*>(router);
-  // a token a cluster while the clusters fit the SMs side by side; beyond that four share the router's rows
-  if (T * sb::mf::kCluster <= sb::sm_count())
-    sb::mf::route_kernel<1><<<T * sb::mf::kCluster, sb::mf::kThreads, smem, st>>>(hp, h_stride, rp, live, w, idx, T, E, H, k, norm);
-  else
-    sb::mf::route_kernel<4><<<(T + 3) / 4 * sb::mf::kCluster, sb::mf::kThreads, smem, st>>>(hp, h_stride, rp, live, w, idx, T, E, H, k, norm);
+  sb::mf::route_kernel<<<(T + sb::mf::kCluster - 1) / sb::mf::kCluster * sb::mf::kCluster, sb::mf::kRouteThreads, sizeof(double) * E, st>>>(
+      static_cast<const __nv_bfloat16*>(h), h_stride, static_cast<const __nv_bfloat16*>(router), live, w, idx, T, E, H, k, norm);
   return cudaGetLastError() == cudaSuccess ? SB_OK : SB_ERR_CUDA;
 }
 
