@@ -61,7 +61,10 @@ SIZES = [  # T, nq, nkv, D, R, interleaved, dtype, layout, scaling
     (40, 2, 1, 64, 20, True, HF, "odd", "none"), (50, 2, 1, 128, 64, True, BF, "transposed", "none"),
     (9, 1, 1, 7, 2, False, BF, "plain", "none"), (11, 2, 1, 192, 192, False, BF, "plain", "none"),
     (5000, 32, 4, 128, 128, False, BF, "plain", "none"), (8001, 14, 2, 64, 32, True, HF, "plain", "none"),
-    (2500, 16, 8, 128, 64, False, FP, "plain", "none"),
+    (2500, 16, 8, 128, 64, False, FP, "plain", "none"), (16000, 6, 1, 128, 64, True, BF, "plain", "yarn"),
+    (12000, 10, 3, 80, 80, False, HF, "strided", "none"), (10000, 8, 4, 96, 24, False, BF, "plain", "llama3"),
+    (4000, 8, 4, 256, 256, True, FP, "plain", "none"), (700, 4, 2, 80, 40, True, BF, "strided", "none"),
+    (4001, 2, 1, 24, 8, False, FP, "plain", "none"), (801, 5, 3, 512, 64, False, HF, "plain", "none"),
 ]
 
 
@@ -139,6 +142,7 @@ CACHE = [  # T, parts, nq, nkv, D, R, interleaved, dtype, normed
     (1, 1, 2, 1, 128, 128, False, BF, True), (64, 4, 32, 4, 128, 128, False, BF, True), (77, 0, 32, 4, 128, 128, False, BF, True),
     (50, 3, 4, 2, 64, 32, True, BF, False), (33, 0, 3, 3, 96, 96, True, HF, False), (20, 2, 2, 1, 40, 24, False, BF, True),
     (19, 0, 2, 1, 24, 10, True, FP, True), (4100, 0, 32, 4, 128, 128, False, BF, True), (600, 8, 4, 4, 256, 128, False, HF, True),
+    (14001, 0, 6, 1, 128, 128, True, BF, False), (9001, 0, 14, 3, 96, 96, False, HF, True),
 ]
 
 
