@@ -32,7 +32,7 @@ from ..models.decoder import CausalLM
 from ..ops import _lib
 from ..ops import attention as attn_ops
 from ..ops import elementwise as ew
-from ..ops import gemm, sampling
+from ..ops import gemm, rotary, sampling
 
 
 @dataclass
@@ -332,11 +332,12 @@ class LLMEngine:
                                                          self.ctx_lens[:n])
         x, h = ew.add_rmsnorm(x, delta, m.p(pre + "ln1"), a.rms_norm_eps)
         qkv = gemm.gemm_nt(h, m.p(pre + "wqkv"), m._p.get(pre + "bqkv"))
-        if a.qk_norm:
-            qkv = m._qk_norm(qkv, i)
-        qkv = ew.rope_(qkv, pos, m.rope_table(self.device), a.num_heads + a.num_kv_heads, a.head_dim)
-        attn_ops.kv_cache_write(qkv, self.k_cache[i], self.v_cache[i], slots, a.num_heads, a.num_kv_heads,
-                                a.head_dim)
+        if a.rotates_in_pass:
+            self._rotate_into_cache(i, qkv, pos, slots, qkv)
+        else:
+            qkv = ew.rope_(qkv, pos, m.rope_table(self.device), a.num_heads + a.num_kv_heads, a.head_dim)
+            attn_ops.kv_cache_write(qkv, self.k_cache[i], self.v_cache[i], slots, a.num_heads, a.num_kv_heads,
+                                    a.head_dim)
         att = attn_ops.attn_decode_paged(qkv, self.k_cache[i], self.v_cache[i], bt, ctx,
                                          a.num_heads, a.num_kv_heads, a.head_dim, max_ctx=self.cfg.max_model_len,
                                          sinks=m._p.get(pre + "sinks"))
@@ -347,11 +348,29 @@ class LLMEngine:
             from ..models.moe import moe_ffn
 
             d = moe_ffn(h, m.p(pre + "router"), m.p(pre + "experts_wgu"), m.p(pre + "experts_wd"),
-                        a.num_experts_per_tok, a.norm_topk_prob, layer=i)
+                        a.num_experts_per_tok, a.norm_topk_prob, layer=i, live=self.active[:n] if st is None else None)
         else:
             act = ew.swiglu(gemm.gemm_nt(h, m.p(pre + "wgu")))
             d = m.row_parallel_linear(act, m.p(pre + "wd"), "prefill_d", 5) if tp else gemm.gemm_nt(act, m.p(pre + "wd"))
         return x, d
+
+    def _rotate_into_cache(self, i: int, x, pos, slots, out):
+        """Norms, rotation and cache rows of layer ``i`` in one launch (``ops/rotary.py``); ``x``: projection rows, or
+        the partial sums of a split projection."""
+        m, a = self.model, self.model.args
+        qn, kn = (m.p(f"layers.{i}.q_norm"), m.p(f"layers.{i}.k_norm")) if a.qk_norm else (None, None)
+        return rotary.qk_rope_cache(x, pos, m.rope_table(self.device), self.k_cache[i], self.v_cache[i], slots, a.num_heads,
+                                    a.num_kv_heads, a.head_dim, q_norm=qn, k_norm=kn, eps=a.rms_norm_eps,
+                                    interleaved=a.rope_interleaved, out=out)
+
+    def _finalize_qkv(self, i: int, part, n_part: int, n: int, qkv) -> None:
+        """Partial sums of the fused QKV projection -> heads in ``qkv`` and their cache rows."""
+        a = self.model.args
+        if a.rotates_in_pass:
+            self._rotate_into_cache(i, part[:n_part], self.positions[:n], self.slots[:n], qkv)
+            return
+        ew.qkv_finalize(part, n_part, self.positions[:n], self.model.rope_table(self.device), qkv, self.k_cache[i],
+                        self.v_cache[i], self.slots[:n], a.num_heads, a.num_kv_heads, a.head_dim)
 
     def _splitk_linear(self, h, w, bias, n):
         """Skinny projection as fp32 split-K partials; returns (partials[P, n, N], n_written)."""
@@ -366,7 +385,6 @@ class LLMEngine:
         split-K, and the partial sums are consumed by the next kernel (norm / RoPE + cache write)."""
         m, a = self.model, self.model.args
         x = sampling.embed(m.p("embed"), self.cur_tokens[:n])  # residual stream, updated in place
-        table = m.rope_table(self.device)
         qkv = torch.empty((n, (a.num_heads + 2 * a.num_kv_heads) * a.head_dim), device=self.device, dtype=x.dtype)
         pending = None
         fused_mlp = a.intermediate_size % 128 == 0 and n >= 32 and os.environ.get("SB_DECODE_FUSED_MLP", "1") != "0"
@@ -381,8 +399,7 @@ class LLMEngine:
             else:
                 h = ew.add_rmsnorm_partials_(x, pending[0], pending[1], m.p(pre + "ln1"), a.rms_norm_eps)
             part, np_ = self._splitk_linear(h, m.p(pre + "wqkv"), m._p.get(pre + "bqkv"), n)
-            ew.qkv_finalize(part, np_, self.positions[:n], table, qkv, self.k_cache[i], self.v_cache[i], self.slots[:n],
-                            a.num_heads, a.num_kv_heads, a.head_dim)
+            self._finalize_qkv(i, part, np_, n, qkv)
             att = attn_ops.attn_decode_paged(qkv, self.k_cache[i], self.v_cache[i], self.block_tables[:n],
                                              self.ctx_lens[:n], a.num_heads, a.num_kv_heads, a.head_dim,
                                              max_ctx=self.cfg.max_model_len)
@@ -432,7 +449,6 @@ class LLMEngine:
         m, a = self.model, self.model.args
         tp = m.tp.size
         x = sampling.embed(m.p("embed"), self.cur_tokens[:n])
-        table = m.rope_table(self.device)
         qkv = torch.empty((n, (a.num_heads + 2 * a.num_kv_heads) * a.head_dim), device=self.device, dtype=x.dtype)
         pending = None
         fused_mlp = a.intermediate_size % 128 == 0 and n >= 32 and os.environ.get("SB_DECODE_FUSED_MLP", "1") != "0"
@@ -443,8 +459,7 @@ class LLMEngine:
             else:
                 h = ew.add_rmsnorm_partials_(x, pending, pending.shape[0], m.p(pre + "ln1"), a.rms_norm_eps)
             part, np_ = self._splitk_linear(h, m.p(pre + "wqkv"), m._p.get(pre + "bqkv"), n)
-            ew.qkv_finalize(part, np_, self.positions[:n], table, qkv, self.k_cache[i], self.v_cache[i], self.slots[:n],
-                            a.num_heads, a.num_kv_heads, a.head_dim)
+            self._finalize_qkv(i, part, np_, n, qkv)
             att = attn_ops.attn_decode_paged(qkv, self.k_cache[i], self.v_cache[i], self.block_tables[:n],
                                              self.ctx_lens[:n], a.num_heads, a.num_kv_heads, a.head_dim,
                                              max_ctx=self.cfg.max_model_len)
@@ -468,7 +483,7 @@ class LLMEngine:
     @torch.no_grad()
     def _decode_once(self, n: int, masked: bool) -> None:
         m, a = self.model, self.model.args
-        plain = not a.num_experts and not a.qk_norm and not a.attention_sinks
+        plain = not a.num_experts and not a.attention_sinks
         if self.is_cuda and self.tp_size > 1 and m.tp.fused and plain:
             return self._decode_once_fused_tp(n, masked)
         if self.is_cuda and self.cfg.fused_decode and plain and self.tp_size == 1:
@@ -640,18 +655,14 @@ class LLMEngine:
         m, a = self.model, self.model.args
         bs = self.cfg.block_size
         dev = self.device
-        ids, pos, slot_list, cu = [], [], [], [0]
-        rows = []
-        full_slots: List[int] = []  # cache slot of every token (cached prefix + new), per sequence, for the prefix path
+        ids: List[int] = []
+        rows, lens = [], []
         q_first: List[int] = []     # number of cached tokens per sequence = first row that carries a query
-        new_rows_in_full: List[int] = []
-        cu_full = [0]
-        any_cached = False
-        for req in reqs:
+        tables = np.zeros((len(reqs), self.max_blocks_per_seq), dtype=np.int32)
+        for k, req in enumerate(reqs):
             toks = req.prompt + req.partial_tokens
             L = len(toks)
-            bt = np.zeros(self.max_blocks_per_seq, dtype=np.int32)
-            nb = self.rt.sbrt_sched_seq_blocks(self.sched, req.sid, bt.ctypes.data, self.max_blocks_per_seq)
+            nb = self.rt.sbrt_sched_seq_blocks(self.sched, req.sid, tables[k].ctypes.data, self.max_blocks_per_seq)
             assert nb >= (L + bs - 1) // bs, "scheduler did not reserve enough blocks"
             req.cached = self.rt.sbrt_sched_seq_cached(self.sched, req.sid)
             # tokens whose key/value blocks are already in the cache are not recomputed (at least one token is)
@@ -659,42 +670,41 @@ class LLMEngine:
             if req.params.prompt_logprobs or self._record:
                 c = 0  # prompt log-probs need every position's hidden state; routing capture every position's router
             c = (c // bs) * bs
-            any_cached = any_cached or c > 0
             slot = self._free_slots.pop()
             req.slot = slot
             self._slot_req[slot] = req
             rows.append(slot)
-            self.block_tables[slot].copy_(_lib.to_device(torch.from_numpy(bt), dev))
-            all_slots = (bt[np.arange(L) // bs] * bs + np.arange(L) % bs).tolist()
             ids.extend(toks[c:])
-            pos.extend(range(c, L))
-            slot_list.extend(all_slots[c:])
-            cu.append(cu[-1] + (L - c))
-            new_rows_in_full.extend(range(cu_full[-1] + c, cu_full[-1] + L))
+            lens.append(L)
             q_first.append(c)
-            full_slots.extend(all_slots)
-            cu_full.append(cu_full[-1] + L)
+        any_cached = any(q_first)
+        cu = np.concatenate([[0], np.cumsum(np.asarray(lens) - np.asarray(q_first))]).tolist()
+        rows_t = torch.tensor(rows, device=dev, dtype=torch.long)
         t_ids = _lib.to_device(torch.tensor(ids, dtype=torch.int32), dev)
-        t_pos = _lib.to_device(torch.tensor(pos, dtype=torch.int32), dev)
-        t_slots = _lib.to_device(torch.tensor(slot_list, dtype=torch.int32), dev)
-        t_cu = _lib.to_device(torch.tensor(cu, dtype=torch.int32), dev)
+        t_tables = _lib.to_device(torch.from_numpy(tables), dev)
+        self.block_tables[rows_t] = t_tables
+        # the cached rows carry no query: the attention kernel skips the query blocks that lie entirely inside them
+        t_lens, t_q_first = _lib.to_device(torch.tensor([lens, q_first], dtype=torch.int32), dev)
+        # positions and slots of the new tokens, from the lengths, on the device
+        lay = attn_ops.paged_layout(t_tables, t_lens, bs, len(ids), starts=t_q_first)
+        t_pos, t_slots, t_cu = lay.positions, lay.slots, lay.cu_seqlens
 
         def sink(layer, qkv):
             attn_ops.kv_cache_write(qkv, self.k_cache[layer], self.v_cache[layer], t_slots, a.num_heads,
                                     a.num_kv_heads, a.head_dim)
+
+        sink.paged = lambda layer: (self.k_cache[layer], self.v_cache[layer], t_slots)
 
         max_len = max(len(r.prompt) + len(r.partial_tokens) for r in reqs)
         attn_fn = None
         if any_cached:
             # Prefix path: the projections and the MLP run on the new tokens only; attention runs over rows that hold
             # the cached prefix's keys/values (gathered from the paged cache) followed by the new tokens' q, k, v.
-            t_full_slots = _lib.to_device(torch.tensor(full_slots, dtype=torch.long), dev)
-            t_new_rows = _lib.to_device(torch.tensor(new_rows_in_full, dtype=torch.long), dev)
-            t_cu_full = _lib.to_device(torch.tensor(cu_full, dtype=torch.int32), dev)
-            # the cached rows carry no query: the attention kernel skips the query blocks that lie entirely inside them
-            t_q_first = _lib.to_device(torch.tensor(q_first, dtype=torch.int32), dev)
+            Tf = sum(lens)
+            full = attn_ops.paged_layout(t_tables, t_lens, bs, Tf)
+            t_full_slots, t_cu_full = full.slots.long(), full.cu_seqlens
+            t_new_rows = lay.rows.long()
             qd, kvd = a.num_heads * a.head_dim, a.num_kv_heads * a.head_dim
-            Tf = len(full_slots)
 
             def attn_fn(layer, qkv):  # noqa: F811 - runs after sink() has written the new keys/values
                 full = torch.zeros((Tf, qd + 2 * kvd), device=dev, dtype=qkv.dtype)
@@ -725,7 +735,6 @@ class LLMEngine:
                 if r.params.prompt_logprobs:
                     r.prompt_logprobs = [None] + plp[cu[k] : cu[k + 1] - 1].tolist()
         logits = gemm.gemm_nt(last.contiguous(), m.lm_head_weight())
-        rows_t = torch.tensor(rows, device=dev, dtype=torch.long)
         # per-slot sampling parameters and counters
         host = lambda f, dt: torch.tensor([f(r) for r in reqs], device=dev, dtype=dt)  # noqa: E731
         self.temperature[rows_t] = host(lambda r: r.params.temperature, torch.float32)

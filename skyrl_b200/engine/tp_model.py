@@ -103,11 +103,7 @@ class TPEngineModel(CausalLM):
         pre = f"layers.{i}."
         x, h = ew.add_rmsnorm(x, delta, self.p(pre + "ln1"), a.rms_norm_eps)
         qkv = gemm.linear(h, self.p(pre + "wqkv"), self._p.get(pre + "bqkv"))
-        if a.qk_norm:
-            qkv = self._qk_norm(qkv, i)
-        qkv = ew.rope(qkv, pos, self.rope_table(qkv.device), a.num_heads + a.num_kv_heads, a.head_dim)
-        if kv_sink is not None:
-            kv_sink(i, qkv)
+        qkv = self._rotate(i, qkv, pos, kv_sink)
         if attn_fn is not None:
             att = attn_fn(i, qkv)
         else:

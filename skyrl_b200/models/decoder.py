@@ -29,8 +29,11 @@ import torch.utils.checkpoint
 
 from ..ops import attention as attn_ops
 from ..ops import elementwise as ew
-from ..ops import gemm
+from ..ops import gemm, rotary
 from ..ops import lm_head as lm_head_ops
+from ..utils.log import get_logger
+
+logger = get_logger(__name__)
 
 
 @dataclass
@@ -45,6 +48,9 @@ class ModelArgs:
     rms_norm_eps: float = 1e-6
     rope_theta: float = 10000.0
     max_position_embeddings: int = 32768
+    rope_scaling: Optional[dict] = None  # linear / llama3 / yarn, as in a checkpoint's configuration (ops/elementwise.py)
+    partial_rotary_factor: float = 1.0  # rotated part of each head
+    rope_interleaved: bool = False  # rotate neighbouring elements (2i, 2i + 1) instead of (i, i + half)
     tie_word_embeddings: bool = False
     attention_bias: bool = False  # Qwen2: bias on q/k/v projections
     qk_norm: bool = False  # Qwen3: per-head RMSNorm on q and k
@@ -71,16 +77,35 @@ class ModelArgs:
     def qkv_dim(self) -> int:
         return self.q_dim + 2 * self.kv_dim
 
+    @property
+    def rotary_dim(self) -> int:
+        return int(self.head_dim * self.partial_rotary_factor) // 2 * 2
+
+    @property
+    def rotates_in_pass(self) -> bool:
+        """Whether the heads go through ``ops/rotary.py``: per-head norms, neighbouring pairs or heads rotated in part."""
+        return self.qk_norm or self.rope_interleaved or self.rotary_dim != self.head_dim
+
     @classmethod
     def from_hf_config(cls, cfg: dict) -> "ModelArgs":
         mt = cfg.get("model_type", "llama")
         heads = cfg["num_attention_heads"]
+        rope = dict(cfg.get("rope_parameters") or cfg.get("rope_scaling") or {})
+        theta = cfg.get("rope_theta", rope.pop("rope_theta", 10000.0))
+        partial = cfg.get("partial_rotary_factor", rope.pop("partial_rotary_factor", 1.0)) or 1.0
+        kind = rope.get("rope_type") or rope.get("type") or "default"
+        if kind not in ("default", "linear", "llama3", "yarn"):
+            logger.warning("rope scaling '%s' is not supported: positions are not scaled", kind)
+        scaling = rope if kind in ("linear", "llama3", "yarn") else None
+        if scaling is not None and kind != "linear":
+            scaling.setdefault("original_max_position_embeddings", cfg.get("max_position_embeddings", 32768))
         return cls(
             vocab_size=cfg["vocab_size"], hidden_size=cfg["hidden_size"], num_layers=cfg["num_hidden_layers"],
             num_heads=heads, num_kv_heads=cfg.get("num_key_value_heads", heads),
             head_dim=cfg.get("head_dim") or cfg["hidden_size"] // heads,
             intermediate_size=cfg.get("intermediate_size", 0), rms_norm_eps=cfg.get("rms_norm_eps", 1e-6),
-            rope_theta=float(cfg.get("rope_theta", 10000.0)),
+            rope_theta=float(theta), rope_scaling=scaling, partial_rotary_factor=float(partial),
+            rope_interleaved=bool(cfg.get("rope_interleaved", False)),
             max_position_embeddings=cfg.get("max_position_embeddings", 32768),
             tie_word_embeddings=bool(cfg.get("tie_word_embeddings", False)),
             attention_bias=bool(cfg.get("attention_bias", mt == "qwen2")), qk_norm=mt in ("qwen3", "qwen3_moe"),
@@ -103,6 +128,12 @@ class ModelArgs:
             "tie_word_embeddings": self.tie_word_embeddings, "attention_bias": self.attention_bias,
             "hidden_act": "silu", "torch_dtype": "bfloat16",
         }  # fmt: skip
+        if self.rope_scaling:
+            cfg["rope_scaling"] = dict(self.rope_scaling)
+        if self.partial_rotary_factor != 1.0:
+            cfg["partial_rotary_factor"] = self.partial_rotary_factor
+        if self.rope_interleaved:
+            cfg["rope_interleaved"] = True
         if self.attention_sinks:
             cfg["attention_sinks"] = True
         if self.num_experts:
@@ -266,30 +297,45 @@ class CausalLM(nn.Module):
 
     def rope_table(self, device) -> torch.Tensor:
         if self._rope_table is None or self._rope_table.device != torch.device(device):
-            self._rope_table = ew.build_rope_table(self.args.max_position_embeddings, self.args.head_dim,
-                                                   self.args.rope_theta, device)
+            a = self.args
+            n = a.max_position_embeddings
+            if a.rope_scaling and "original_max_position_embeddings" in a.rope_scaling:  # the stretched context
+                n = max(n, int(a.rope_scaling["original_max_position_embeddings"] * float(a.rope_scaling["factor"])))
+            self._rope_table = ew.build_rope_table(n, a.rotary_dim, a.rope_theta, device, scaling=a.rope_scaling)
         return self._rope_table
 
     # ------------------------------------------------------------------ forward
-    def _qk_norm(self, qkv: torch.Tensor, i: int) -> torch.Tensor:
+    def _rotate(self, i: int, qkv: torch.Tensor, pos: torch.Tensor, kv_sink=None, heads: Optional[Tuple[int, int]] = None):
+        """Fused projection rows -> normed (where the model has per-head norms) and rotated heads, handed to ``kv_sink``.
+        ``heads``: query and key heads of the rows where they are not all of the model's.  A sink with a ``paged(layer)``
+        method (key cache, value cache, slots) gets its cache rows from the same launch; no gradients then."""
         a = self.args
-        T = qkv.shape[0]
-        q = qkv[:, : a.q_dim].reshape(T * a.num_heads, a.head_dim)
-        k = qkv[:, a.q_dim : a.q_dim + a.kv_dim].reshape(T * a.num_kv_heads, a.head_dim)
-        q = ew.rmsnorm(q, self.p(f"layers.{i}.q_norm"), a.rms_norm_eps).reshape(T, a.q_dim)
-        k = ew.rmsnorm(k, self.p(f"layers.{i}.k_norm"), a.rms_norm_eps).reshape(T, a.kv_dim)
-        return torch.cat([q, k, qkv[:, a.q_dim + a.kv_dim :]], dim=-1)
+        nq, nkv = heads or (a.num_heads, a.num_kv_heads)
+        table = self.rope_table(qkv.device)
+        if a.rotates_in_pass:
+            pos = pos.to(torch.int32)
+            qn, kn = (self.p(f"layers.{i}.q_norm"), self.p(f"layers.{i}.k_norm")) if a.qk_norm else (None, None)
+            if hasattr(kv_sink, "paged"):
+                k, v, slots = kv_sink.paged(i)
+                return rotary.qk_rope_cache(qkv, pos, table, k, v, slots, nq, nkv, a.head_dim, q_norm=qn, k_norm=kn,
+                                            eps=a.rms_norm_eps, interleaved=a.rope_interleaved, out=qkv)
+            if a.qk_norm:
+                qkv = rotary.qk_norm_rope(qkv, qn, kn, pos, table, nq, nkv, a.head_dim, a.rms_norm_eps,
+                                          interleaved=a.rope_interleaved)
+            else:
+                qkv = rotary.rotary(qkv, pos, table, nq + nkv, a.head_dim, interleaved=a.rope_interleaved)
+        else:
+            qkv = ew.rope(qkv, pos, table, nq + nkv, a.head_dim)
+        if kv_sink is not None:
+            kv_sink(i, qkv)
+        return qkv
 
     def _layer(self, i: int, x, delta, pos, cu, max_seqlen, kv_sink=None, attn_fn=None):
         a = self.args
         pre = f"layers.{i}."
         x, h = ew.add_rmsnorm(x, delta, self.p(pre + "ln1"), a.rms_norm_eps)
         qkv = gemm.linear(h, self.p(pre + "wqkv"), self._p.get(pre + "bqkv"))
-        if a.qk_norm:
-            qkv = self._qk_norm(qkv, i)
-        qkv = ew.rope(qkv, pos, self.rope_table(qkv.device), a.num_heads + a.num_kv_heads, a.head_dim)
-        if kv_sink is not None:
-            kv_sink(i, qkv)
+        qkv = self._rotate(i, qkv, pos, kv_sink)
         if attn_fn is not None:  # the caller supplies attention (e.g. over cached key/value prefixes)
             att = attn_fn(i, qkv)
         else:

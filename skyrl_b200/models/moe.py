@@ -14,6 +14,12 @@ import torch
 from ..ops import elementwise as ew
 from ..ops import gemm  # noqa: F401
 from ..ops import grouped_gemm as gg
+from ..ops import moe_few
+
+# Up to this many rows an expert in the mean, and without gradients, the layer runs on ``ops/moe_few.py``.  Layer times
+# there / through the grouped GEMMs in us: 128 experts of 2048 x 768, top 8: 191 / 362 at 64 tokens (4 rows), 326 / 368 at
+# 256 (16 rows); 8 experts of 2048 x 4096, top 2: 115 / 164 at 64 tokens (16 rows), 178 / 154 at 128 (32 rows).
+FEW_ROWS = 16
 
 
 class _RouteFn(torch.autograd.Function):
@@ -69,23 +75,41 @@ def route_topk(h: torch.Tensor, router_w: torch.Tensor, top_k: int, norm_topk_pr
     return w, idx
 
 
+def _takes_few(h, router_w, wgu, wd, top_k) -> bool:
+    if not h.is_cuda or h.shape[0] * top_k > FEW_ROWS * wgu.shape[0] or h.dtype != torch.bfloat16:
+        return False
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (h, router_w, wgu, wd)):
+        return False
+    if not all(t.dtype == h.dtype and t.is_contiguous() for t in (router_w, wgu, wd)):
+        return False
+    return moe_few.supports(h.shape[0], wgu.shape[0], top_k, h.shape[1], wd.shape[2])
+
+
 def moe_ffn(h: torch.Tensor, router_w: torch.Tensor, wgu: torch.Tensor, wd: torch.Tensor, top_k: int,
-            norm_topk_prob: bool = True, routed_indices: torch.Tensor | None = None, layer: int | None = None, qat=None) -> torch.Tensor:
+            norm_topk_prob: bool = True, routed_indices: torch.Tensor | None = None, layer: int | None = None, qat=None,
+            live: torch.Tensor | None = None) -> torch.Tensor:
     """``h``: [T, H]; ``wgu``: [E, 2F, H]; ``wd``: [E, H, F].  ``routed_indices`` replays rollout-time routing;
-    with ``layer`` given, an active ``router_replay`` context records or overrides the choice."""
+    with ``layer`` given, an active ``router_replay`` context records or overrides the choice.  ``live`` ([T] int32):
+    rows whose result is not used where it is 0; on the path for few tokens they read no expert and come out zero."""
     T, H = h.shape
     E = wgu.shape[0]
-    w, idx = route_topk(h, router_w, top_k, norm_topk_prob)
+    few = _takes_few(h, router_w, wgu, wd, top_k)
+    if few:
+        w, idx = moe_few.route_few(h, router_w, top_k, norm_topk_prob, live=live)
+    else:
+        w, idx = route_topk(h, router_w, top_k, norm_topk_prob)
     if layer is not None and routed_indices is None:
         from . import router_replay
 
-        routed_indices = router_replay.on_route(layer, idx)
+        routed_indices = router_replay.on_route(layer, idx.long())
     if routed_indices is not None:
         probs = torch.softmax(h.float() @ router_w.float().t(), dim=-1)
         idx = routed_indices.long()
         w = probs.gather(-1, idx)
         if norm_topk_prob:
             w = w / w.sum(dim=-1, keepdim=True)
+    if few:
+        return moe_few.expert_ffn_few(h, w.float().contiguous(), idx.to(torch.int32).contiguous(), wgu, wd)
     plan = gg.plan_groups(idx.reshape(-1), E, top_k)
     # rows grouped by expert, every expert's range padded to whole 128-row tiles (padding rows are zero)
     x = gg.dispatch_rows(h, plan)
