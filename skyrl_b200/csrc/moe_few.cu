@@ -77,6 +77,7 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = static_cast<int>(blockIdx.x / kCluster) * kCluster;
   cluster.barrier_arrive();
+  pdl_launch_dependents();
   if (threadIdx.x == 0) n_cand = 0;
   const int per = (E + kCluster - 1) / kCluster;
   const int e_hi = min(E, (rank + 1) * per);
@@ -201,7 +202,7 @@ __host__ __device__ constexpr int lists_bytes(int n, int E) {
   return (4 * 3 * 32 + 4 * E + 2 * (E + 1) * 2 + 2 * E + 2 * n + 127) / 128 * 128;
  }
 
-__device__ __forceinline__ Lists build_lists(char* smem, const int* __restrict__ idx, int n, int E) {
+__device__ __forceinline__ Lists build_lists(char* smem, const int* idx, int n, int E) {
   Lists L;
   L.count = reinterpret_cast<int*>(smem);
   L.cursor = L.count + 3 * 32;
@@ -210,10 +211,11 @@ __device__ __forceinline__ Lists build_lists(char* smem, const int* __restrict__
   L.used = L.unit0 + E + 1;
   L.entry = L.used + E;
   const int lane = threadIdx.x & 31;
+  const int held = threadIdx.x < n ? idx[threadIdx.x] : -1;  // this thread's first entry
   for (int e = threadIdx.x; e < E; e += blockDim.x) L.cursor[e] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int e = idx[i];
+    const int e = i == threadIdx.x ? held : idx[i];
     if (e >= 0 && e < E) atomicAdd(&L.cursor[e], 1);
   }
   __syncthreads();
@@ -269,7 +271,7 @@ __device__ __forceinline__ Lists build_lists(char* smem, const int* __restrict__
   __syncthreads();
   if (L.n_units == L.n_used) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const int e = idx[i];
+      const int e = i == threadIdx.x ? held : idx[i];
       if (e >= 0 && e < E) L.entry[atomicAdd(&L.cursor[e], 1)] = static_cast<unsigned short>(i);
     }
   } else if (threadIdx.x < 32) {  // in the entries' order, 32 at a time
@@ -295,6 +297,7 @@ struct Unit {
 };
 __device__ __forceinline__ Unit unit_at(const Lists& L, int unit) {
   int lo = 0, hi = L.n_used - 1;  // last used expert whose first unit is not behind `unit`
+  if (L.n_units == L.n_used) lo = hi = unit;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (L.unit0[mid] <= unit)
@@ -406,6 +409,7 @@ __device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red
   };
   Turn turn;
   int r0 = -1;
+  bool ok = true;  // after a wait gave up, the items are run through without waiting: every warp still meets the others
   for (int i = 0; i < items; ++i) {
     const Unit u = unit_of();
     float acc[kNt][4];
@@ -428,11 +432,11 @@ __device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red
       const int off = g * 2 * s.piece + lo * 64 + 16 * t4;
       const char* top = buf + static_cast<size_t>(turn.stage) * 16 * s.piece + off;
       uint64_t* free_a = &ring.empty[turn.stage];
-      if (!mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d02)) return;
+      ok = ok && mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d02);
       turn.step(s.stages);
       const char* low = buf + static_cast<size_t>(turn.stage) * 16 * s.piece + off;
       uint64_t* free_b = &ring.empty[turn.stage];
-      if (!mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d03)) return;
+      ok = ok && mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d03);
       turn.step(s.stages);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
@@ -496,13 +500,14 @@ __device__ __forceinline__ void ring_drain(Ring& ring, const Shape& s, Turn turn
 // ---------------------------------------------------------------------------
 template <int kSteps>
 __global__ void __launch_bounds__(kRingThreads, 1)
-gate_up_kernel(const __nv_bfloat16* h, long long h_stride, const int* __restrict__ idx, const __nv_bfloat16* __restrict__ wgu,
+gate_up_kernel(const __nv_bfloat16* h, long long h_stride, const int* idx, const __nv_bfloat16* __restrict__ wgu,
                __nv_bfloat16* act, int n, int k, int E, int H, int F, Shape s, int* status) {
   __shared__ Ring ring;
   extern __shared__ __align__(128) char smem[];
   float4* red = reinterpret_cast<float4*>(smem);
   char* buf = smem + kRedBytes;
   ring_init(ring, s.stages);
+  pdl_wait();
   const Lists L = build_lists(buf + static_cast<size_t>(s.stages) * 16 * s.piece, idx, n, E);
   const int tiles = (F + 7) >> 3;
   const long long items = static_cast<long long>(L.n_units) * tiles;
@@ -673,10 +678,8 @@ cudaError_t launch_gate_up(const void* h, long long h_stride, const int* idx, co
     if (e != cudaSuccess) return e;
     attr = true;
   }
-  gate_up_kernel<kSteps><<<sm_count(), kRingThreads, smem, st>>>(static_cast<const __nv_bfloat16*>(h), h_stride, idx,
-                                                                 static_cast<const __nv_bfloat16*>(wgu), static_cast<__nv_bfloat16*>(act),
-                                                                 T * k, k, E, H, F, s, status);
-  return cudaGetLastError();
+  return launch_pdl(gate_up_kernel<kSteps>, dim3(sm_count()), dim3(kRingThreads), smem, st, static_cast<const __nv_bfloat16*>(h), h_stride,
+                    idx, static_cast<const __nv_bfloat16*>(wgu), static_cast<__nv_bfloat16*>(act), T * k, k, E, H, F, s, status);
 }
 
 cudaError_t launch_down(const void* act, const int* idx, const float* w, const void* wd, void* out, int T, int k, int E, int H, int F,

@@ -29,8 +29,7 @@ __device__ __forceinline__ long long layout_block_sum(long long v, long long* re
 }
 
 __global__ void __launch_bounds__(kLayoutThreads)
-paged_layout_kernel(const int* __restrict__ tables, long long table_stride, int width, const int* __restrict__ starts,
-                    const int* __restrict__ lens, int B, int bs, int total, int* __restrict__ cu, int* __restrict__ pos,
+paged_layout_kernel(const int* tables, long long table_stride, int width, const int* starts, const int* lens, int B, int bs, int total, int* __restrict__ cu, int* __restrict__ pos,
                     int* __restrict__ slots, int* __restrict__ whole) {
   __shared__ long long red[kLayoutThreads / 32];
   pdl_launch_dependents();
@@ -61,7 +60,7 @@ paged_layout_kernel(const int* __restrict__ tables, long long table_stride, int 
     if (rows + r >= total) break;
     const int p = s + static_cast<int>(r);
     const int blk = p / bs;
-    const int e = blk < width ? __ldg(table + blk) : -1;
+    const int e = blk < width ? table[blk] : -1;
     const long long slot = e >= 0 ? static_cast<long long>(e) * bs + (p - blk * bs) : -1;
     pos[rows + r] = p;
     slots[rows + r] = slot > 0x7fffffffLL ? -1 : static_cast<int>(slot);

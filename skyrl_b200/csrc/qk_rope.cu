@@ -117,6 +117,18 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Partial sums are added up in two fp32 words, rounded to fp32 and then, as an unsplit projection's sum would be, to the
+// rows' type: the result does not depend on how many parts it came in.
+struct Sum {
+  float hi = 0.f, lo = 0.f;
+  __device__ __forceinline__ void add(float v) {
+    const float s = hi + v, b = s - hi;
+    lo += (hi - (s - b)) + (v - b);  // what the addition rounded away
+    hi = s;
+  }
+  __device__ __forceinline__ float get() const { return hi + lo; }
+};
+
 // Sum over the 1 << lg consecutive lanes of a head.
 __device__ __forceinline__ float group_sum(float v, int lg) {
 #pragma unroll
@@ -191,7 +203,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
   Vec8<T> vlo, vhi;
   if (on) {
     if (kPart) {
-      float lo[8] = {}, hi[8] = {};
+      Sum lo[8], hi[8];
       const float* p = static_cast<const float*>(a.src) + static_cast<size_t>(t) * a.src_stride + h * a.D;
       for (int i = 0; i < a.n_part; ++i, p += a.part_stride) {
         Vec8<float> l, r;
@@ -202,13 +214,19 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
         r.get(fr);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          lo[j] += fl[j];
-          hi[j] += fr[j];
+          lo[j].add(fl[j]);
+          hi[j].add(fr[j]);
         }
       }
+      float fl[8], fr[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        fl[j] = lo[j].get();
+        fr[j] = hi[j].get();
+      }
       // the unsplit projection stores its rows in this type: keep that rounding, so that both paths agree
-      vlo.set(lo);
-      vhi.set(hi);
+      vlo.set(fl);
+      vhi.set(fr);
     } else {
       const T* p = static_cast<const T*>(a.src) + static_cast<size_t>(t) * a.src_stride + h * a.D;
       vlo.load(p + u.lo);
@@ -216,8 +234,8 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
     }
   }
   float cs[8], sn[8];
-  if (u.rot) load_angles(a.table, __ldg(a.pos + t), a.max_pos, a.R, c, cs, sn);
-  long long slot = a.slots ? __ldg(a.slots + t) : -1;
+  if (u.rot) load_angles(a.table, a.pos[t], a.max_pos, a.R, c, cs, sn);
+  long long slot = a.slots ? a.slots[t] : -1;
   if (slot >= a.n_slots) slot = -1;
   float e[16];
   float ss = 0.f;
@@ -308,7 +326,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(const Args a) {
         dhi.get(g + 8);
         if (u.rot) {
           float cs[8], sn[8];
-          load_angles(a.table, __ldg(a.pos + t), a.max_pos, a.R, c, cs, sn);
+          load_angles(a.table, a.pos[t], a.max_pos, a.R, c, cs, sn);
           rotate16<kInter>(g, cs, sn, -1.f);
         }
 #pragma unroll
@@ -581,9 +599,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     sin_next = __ldg(reinterpret_cast<const float4*>(t + (a.R >> 1)));
   };
   int p_next = 0;
-  if (count > 0) angles(__ldg(a.pos + at.t));
+  if (count > 0) angles(a.pos[at.t]);
   advance(at);
-  if (count > 1) p_next = __ldg(a.pos + at.t);
+  if (count > 1) p_next = a.pos[at.t];
   advance(at);
 
   f2 acc_q[4] = {0ull, 0ull, 0ull, 0ull}, acc_k[4] = {0ull, 0ull, 0ull, 0ull};  // weight gradients: a's, then b's
@@ -599,12 +617,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     const f2 ss[2] = {pack2(sin_next.x * sg, sin_next.y * sg), pack2(sin_next.z * sg, sin_next.w * sg)};
     const f2 ns[2] = {pack2(sin_next.x * -sg, sin_next.y * -sg), pack2(sin_next.z * -sg, sin_next.w * -sg)};
     if (i + 1 < count) angles(p_next);
-    if (i + 2 < count) p_next = __ldg(a.pos + at.t);
+    if (i + 2 < count) p_next = a.pos[at.t];
     advance(at);
     const int t = now.t, h0 = now.blk * block_heads, h1 = min(a.heads, h0 + block_heads);
     advance(now);
     long long slot = -1;
-    if (!kBack && a.slots) slot = __ldg(a.slots + t);
+    if (!kBack && a.slots) slot = a.slots[t];
     char* piece = mine + stage * stage_bytes;
     if (!mbar_wait(&bar[stage], parity, status, 0x4d10)) {
       ok = false;
@@ -659,16 +677,17 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
         const f2 r2 = pack2(r, r);
         __syncwarp();  // every lane has read its elements before one that goes along with it writes them
         if (kBack) {
-          const float back = -m * inv_d * r * r * r;  // - mean(dn w xh) * rstd^2
+          const float back = -m * inv_d * r * r;  // - mean(dn w xh) * rstd
           const f2 b2 = pack2(back, back);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
+            const f2 xa = mul2(x.a[j], r2), xb = mul2(x.b[j], r2);  // xh
             if (on) {
-              acc[j] = fma2(mul2(v.a[j], x.a[j]), r2, acc[j]);
-              acc[2 + j] = fma2(mul2(v.b[j], x.b[j]), r2, acc[2 + j]);
+              acc[j] = fma2(v.a[j], xa, acc[j]);
+              acc[2 + j] = fma2(v.b[j], xb, acc[2 + j]);
             }
-            v.a[j] = fma2(x.a[j], b2, mul2(mul2(v.a[j], wt.a[j]), r2));
-            v.b[j] = fma2(x.b[j], b2, mul2(mul2(v.b[j], wt.b[j]), r2));
+            v.a[j] = fma2(xa, b2, mul2(mul2(v.a[j], wt.a[j]), r2));
+            v.b[j] = fma2(xb, b2, mul2(mul2(v.b[j], wt.b[j]), r2));
           }
         } else {
 #pragma unroll
@@ -770,9 +789,9 @@ template <typename T, bool kPart>
 __device__ __forceinline__ float elem(const Args& a, int t, int h, int e) {
   if (kPart) {
     const float* p = static_cast<const float*>(a.src) + static_cast<size_t>(t) * a.src_stride + h * a.D + e;
-    float v = 0.f;
-    for (int i = 0; i < a.n_part; ++i) v += p[static_cast<size_t>(i) * a.part_stride];
-    return to_f(from_f<T>(v));
+    Sum v;
+    for (int i = 0; i < a.n_part; ++i) v.add(p[static_cast<size_t>(i) * a.part_stride]);
+    return to_f(from_f<T>(v.get()));
   }
   return to_f(static_cast<const T*>(a.src)[static_cast<size_t>(t) * a.src_stride + h * a.D + e]);
 }

@@ -250,7 +250,7 @@ def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cac
     outside the cache, such as -1, writes nothing; two rows must not share a slot).
 
     ``x``: ``[T, (nq + 2 nkv) * head_dim]`` in the caches' type, or the fp32 partial sums ``[P, T, ...]`` of a split
-    projection, which are summed and rounded to that type first.  Caches: ``[blocks, block_size, nkv, head_dim]``.
+    projection, which are summed (no sum's rounding shows) and rounded to that type first.  Caches: ``[blocks, block_size, nkv, head_dim]``.
     Returns the rows, in ``out`` when given; ``out`` may be ``x`` itself."""
     what = "qk_rope_cache"
     if x.dim() not in (2, 3):
@@ -281,7 +281,7 @@ def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cac
                             or (T > 1 and out.stride(0) < W)):
         raise ValueError(f"{what}: out must be [{T}, {W}] rows in the caches' type")
     if not x.is_cuda:
-        rows = x.sum(0).to(dt) if partial else x
+        rows = x.double().sum(0).float().to(dt) if partial else x
         res = _fwd_ref(rows, q_norm, k_norm, pos, table, nq, nkv, head_dim, eps, interleaved, 1.0)
         keep = (slots >= 0) & (slots < k_cache.shape[0] * k_cache.shape[1])
         at = slots[keep].long()

@@ -148,7 +148,7 @@ def test_cache_rows_partial_sums_and_empty_slots():
     T, nq, nkv, D, bs = 9, 3, 2, 16, 4
     W = (nq + 2 * nkv) * D
     part = torch.randn(3, T, W, generator=g)
-    x = part.sum(0)
+    x = part.double().sum(0).float()
     qw, kw = (1 + 0.2 * torch.randn(D, generator=g) for _ in range(2))
     pos, table = torch.arange(T, dtype=torch.int32) * 3, ew.build_rope_table(64, D, 1e4, "cpu")
     slots = torch.tensor([5, -1, 0, 19, 20, 7, -5, 2, 11], dtype=torch.int32)  # 20 lies behind the cache

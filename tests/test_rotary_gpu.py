@@ -156,10 +156,7 @@ def test_cache_rows(T, parts, nq, nkv, D, R, inter, dtype, normed):
     src = x
     if parts:
         src = torch.randn(parts, T, W, generator=g, device="cuda")
-        acc = torch.zeros(T, W, device="cuda")
-        for p in src:  # the kernel's order
-            acc += p
-        x = acc.to(dtype)
+        x = src.double().sum(0).float().to(dtype)  # a sum that has lost nothing, in fp32 and then in the rows' type
     blocks = T // bs + 2
     slots = torch.randperm(blocks * bs, generator=g, device="cuda")[:T].to(torch.int32)
     if T > 4:
