@@ -85,8 +85,8 @@ def route_few(h: torch.Tensor, router_w: torch.Tensor, top_k: int, norm_topk_pro
             off = (live == 0)[:, None]
             w, idx = torch.where(off, torch.zeros_like(w), w), torch.where(off, torch.full_like(idx, -1), idx)
         return w, idx
-    w = torch.empty((T, top_k), device=h.device, dtype=torch.float32)
-    idx = torch.empty((T, top_k), device=h.device, dtype=torch.int32)
+    w = h.new_empty((T, top_k), dtype=torch.float32)
+    idx = torch.empty_like(w, dtype=torch.int32)
     if T == 0:
         return w, idx
     h = _rows(h)

@@ -194,20 +194,27 @@ def _launch_bwd(dy, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, 
     dy = _row_major(dy)
     T, W = x.shape
     dx = _rows_like(x)
-    wanted = [(g, w) for g, w, on in zip(main_grads, (q_norm, k_norm), want) if on]
-    # added in place where every wanted gradient has its fp32 buffer, stored in the weights' type where none has; a mix
-    # goes through fp32 zeros
-    direct = bool(wanted) and all(g is not None and g.is_contiguous() and g.dtype == torch.float32 for g, _ in wanted)
-    mixed = not direct and any(g is not None for g, _ in wanted)
-    dqw, dkw = [None if not on else g if direct else torch.zeros_like(w, dtype=torch.float32) if mixed else torch.empty_like(w)
-                for g, w, on in zip(main_grads, (q_norm, k_norm), want)]
+    want_q, want_k = want
+    mq, mk = main_grads[0] if want_q else None, main_grads[1] if want_k else None
+    direct = mixed = False
+    if mq is None and mk is None:  # stored in the weights' type
+        dqw, dkw = torch.empty_like(q_norm) if want_q else None, torch.empty_like(k_norm) if want_k else None
+    else:
+        # added in place where every wanted gradient has its fp32 buffer; a mix goes through fp32 zeros
+        direct = all(g is not None and g.is_contiguous() and g.dtype == torch.float32
+                     for g, on in ((mq, want_q), (mk, want_k)) if on)
+        mixed = not direct
+        dqw, dkw = (mq, mk) if direct else (torch.zeros_like(w, dtype=torch.float32) if on else None
+                                            for w, on in ((q_norm, want_q), (k_norm, want_k)))
     if T == 0:
         return (dx, *(None if direct or g is None else g.zero_() for g in (dqw, dkw)))
     lib = _k()
     max_pos, R = table.shape
     heads = W // D
+    part = None
     n_parts = lib.sb_qk_norm_rope_bwd_parts(T, heads, D)
-    part = torch.empty(n_parts * 2 * D, device=x.device, dtype=torch.float32) if wanted else None
+    if want_q or want_k:
+        part = torch.empty(n_parts * 2 * D, device=x.device, dtype=torch.float32)
     code = _lib.call_on(
         x.get_device(), lib.sb_qk_norm_rope_bwd, dy.data_ptr(), x.data_ptr(), dx.data_ptr(), q_norm.data_ptr(),
         k_norm.data_ptr(), pos.data_ptr(), table.data_ptr(), None if dqw is None else dqw.data_ptr(),
@@ -259,7 +266,7 @@ def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cac
     dt = k_cache.dtype
     if dt not in _DTYPE or v_cache.dtype != dt or x.dtype != (torch.float32 if partial else dt):
         raise ValueError(f"{what}: rows {x.dtype} and caches {dt}, {v_cache.dtype} do not go together")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} has no gradient: use qk_norm_rope or rotary where one is needed")
     _check(x, pos, table, nq, nkv, head_dim, q_norm, k_norm, what)
     T, W = x.shape[-2:]
@@ -269,10 +276,11 @@ def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cac
         raise ValueError(f"{what}: partial sums must be rows of unit stride")
     if q_norm is not None and (q_norm.dtype != dt or k_norm.dtype != dt):
         raise ValueError(f"{what}: norm weights must have the caches' type")
-    if k_cache.shape != v_cache.shape or k_cache.shape[2:] != (nkv, head_dim):
-        raise ValueError(f"{what}: caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} do not hold {nkv} heads of size {head_dim}")
-    if not k_cache.is_contiguous() or not v_cache.is_contiguous() or k_cache.dim() != 4:
-        raise ValueError(f"{what}: caches must be contiguous [blocks, block_size, heads, head_dim] tensors")
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[2] != nkv or shape[3] != head_dim or v_cache.shape != shape:
+        raise ValueError(f"{what}: caches {tuple(shape)}, {tuple(v_cache.shape)} do not hold {nkv} heads of size {head_dim}")
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise ValueError(f"{what}: caches must be contiguous")
     if slots.dtype != torch.int32 or slots.dim() != 1 or slots.numel() != T or not slots.is_contiguous():
         raise ValueError(f"{what}: slots must be a contiguous int32 [{T}] tensor")
     if not (k_cache.get_device() == v_cache.get_device() == slots.get_device() == x.get_device()):
