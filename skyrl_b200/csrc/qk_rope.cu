@@ -576,16 +576,19 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     if (kBack && nx > 0)
       bulk_load(dst + piece_bytes, static_cast<const T*>(a.x) + static_cast<size_t>(p.t) * a.x_stride + h0 * a.D, nx, &bar[stage]);
   };
-  Place now, ahead;  // the piece in work, the piece to be loaded next
+  Place now, ahead, at;  // the piece in work, the one to be loaded next, the one whose position is read next
   now.t = first / a.blocks_per_row;
   now.blk = first - now.t * a.blocks_per_row;
-  ahead = now;
+  ahead = at = now;
+  const int p_first = count > 0 ? a.pos[at.t] : 0;
+  advance(at);
+  int p_next = count > 1 ? a.pos[at.t] : 0;
+  advance(at);
   for (int i = 0; i < kStages - 1; ++i) {
     if (lane == 0 && i < count) fill(ahead, i);
     advance(ahead);
   }
   // angles of the next piece and the position of the one after it are under way while a piece is in work
-  Place at = now;
   float4 cos_next = make_float4(1.f, 1.f, 1.f, 1.f), sin_next = make_float4(0.f, 0.f, 0.f, 0.f);
   auto angles = [&](int p) {
     if (!rot) return;
@@ -598,11 +601,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     cos_next = __ldg(reinterpret_cast<const float4*>(t));
     sin_next = __ldg(reinterpret_cast<const float4*>(t + (a.R >> 1)));
   };
-  int p_next = 0;
-  if (count > 0) angles(a.pos[at.t]);
-  advance(at);
-  if (count > 1) p_next = a.pos[at.t];
-  advance(at);
+  if (count > 0) angles(p_first);
 
   f2 acc_q[4] = {0ull, 0ull, 0ull, 0ull}, acc_k[4] = {0ull, 0ull, 0ull, 0ull};  // weight gradients: a's, then b's
   const float inv_d = 1.f / static_cast<float>(a.D);
@@ -743,7 +742,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
           if (globaltimer_ns() - t0 > kWaitTimeoutNs) break;
       }
     }
-    tma_store_wait<0>();
+    tma_store_wait_read<0>();  // the buffers have been read; the writes end with the kernel
   }
   if (!kBack || !a.dw_part) return;
   // lanes that own the same elements of different heads, then the warps, in a fixed order
@@ -970,7 +969,7 @@ constexpr int kRowSmem = 200 * 1024;
 template <typename T, bool kInter, Mode kMode>
 cudaError_t launch_rows(Args a, int ctas, cudaStream_t st) {
   const int head = a.D * static_cast<int>(sizeof(T)), per_head = kRowWarps * kStages * head * (kMode == kNormBack ? 2 : 1);
-  int block = kRowSmem / per_head;
+  int block = kRowSmem / per_head;  // as large as the buffers allow, and alike
   a.blocks_per_row = (a.heads + block - 1) / block;
   block = (a.heads + a.blocks_per_row - 1) / a.blocks_per_row;
   const size_t sums = kMode == kNormBack ? sizeof(float) * kRowWarps * 2 * a.D : 0;
@@ -989,10 +988,10 @@ cudaError_t launch_rows(Args a, int ctas, cudaStream_t st) {
   return launch_pdl(rows_kernel<T, kInter, kMode>, dim3(ctas), dim3(kRowWarps * 32), smem, st, a, block * head, status);
 }
 
-// From how many bytes of rows on the pipeline is taken.  Below, its start (5 us against 2) costs more than it gains, and
+// From how many bytes of rows on the pipeline is taken.  Below, its start (4 us against 2) costs more than it gains, and
 // rows that lie in L2 come fast enough through plain loads.  bf16, 40 heads of 128, plain kernel / pipeline in us: forward
-// of 23 MB 12.1 / 13.5, of 47 MB 27.9 / 23.4, of 160 MB 88.8 / 59.9; backward of 0.6 MB 6.7 / 7.7, of 1.5 MB 11.7 / 7.7, of
-// 160 MB 216 / 89.5.
+// of 23 MB 12.1 / 13.5, of 47 MB 28.3 / 23.5, of 160 MB 89.7 / 60.0; backward of 0.6 MB 6.2 / 6.8, of 1.5 MB 8.7 / 7.0, of
+// 160 MB 144 / 90.
 constexpr long long kForwardFrom = 28LL << 20, kBackwardFrom = 640LL << 10;
 bool row_pipeline(const Args& a, size_t elt, long long from) {
   return a.D <= 256 && vectorised(a, elt, 8) && static_cast<long long>(a.T) * a.heads * a.D * static_cast<long long>(elt) > from;
