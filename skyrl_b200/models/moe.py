@@ -105,7 +105,7 @@ def moe_ffn(h: torch.Tensor, router_w: torch.Tensor, wgu: torch.Tensor, wd: torc
     if routed_indices is not None:
         probs = torch.softmax(h.float() @ router_w.float().t(), dim=-1)
         idx = routed_indices.long()
-        w = probs.gather(-1, idx)
+        w = probs.gather(-1, idx.clamp_min(0) if few else idx)  # a dead row without a replayed choice keeps its -1
         if norm_topk_prob:
             w = w / w.sum(dim=-1, keepdim=True)
     if few:

@@ -139,3 +139,22 @@ def test_expert_layer_paths_agree_and_dead_rows_are_zero():
     hg = h.clone().requires_grad_()
     moe.moe_ffn(hg, rw, wgu, wd, k).float().sum().backward()
     assert hg.grad is not None and torch.isfinite(hg.grad).all()
+
+
+def test_replayed_routing_with_gaps_and_dead_rows():
+    """Rows without a replayed choice keep their own; a dead row has none and comes out zero."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    T, E, k, H, F = 6, 8, 2, 64, 32
+    h, rw, wgu, wd = r(T, H), r(E, H), r(E, 2 * F, H) / 8, r(E, H, F) / 8
+    live = torch.tensor([1, 0, 1, 0, 1, 1], device="cuda", dtype=torch.int32)
+    routes = torch.randint(0, E, (T, 1, k), generator=g, device="cuda", dtype=torch.int16)
+    routes[1], routes[2] = router_replay.PAD, router_replay.PAD
+    with torch.no_grad(), router_replay.replay_routing(routes):
+        out = moe.moe_ffn(h, rw, wgu, wd, k, layer=0, live=live)
+    with torch.no_grad():
+        own = moe.moe_ffn(h, rw, wgu, wd, k, layer=0)
+        forced = moe.moe_ffn(h, rw, wgu, wd, k, routed_indices=routes[:, 0].clamp_min(0))
+    assert not out[1].any() and torch.equal(out[[0, 3, 4, 5]], forced[[0, 3, 4, 5]])
+    # the row's own weights are taken from the replay's softmax (2^-20 of a weight apart, then one bf16 rounding)
+    assert ((out[2] - own[2]).abs() <= 2.0**-7 * own[2].abs().max()).all() and torch.isfinite(out).all()
