@@ -5,12 +5,14 @@
 //
 // Bound by HBM: with few rows an expert, a layer reads the weights of the experts that some token picked, once, and
 // little else (6 F H bytes an expert).  Rows are not padded or gathered: an expert's rows are a list of (token, slot)
-// entries that every CTA derives from the routing table in shared memory.  The weights stream from global memory into
-// registers as the A operand of m16n8k16 products, eight rows of an expert as its N side.  Such a product is far from
-// bound by the tensor pipe (8 rows: 16 FLOP per weight byte), so what counts is that the operand needs no staging: a
-// lane's 16-byte load of eight consecutive k is used as the fragments of two products whose k order is permuted the
-// same way in both operands, which a sum over k does not see.
-// Every result is summed in a fixed order, without atomics on floats.
+// entries that every CTA derives from the routing table in shared memory.  The weights are the A operand of m16n8k16
+// products, eight rows of an expert the N side.  Such a product is far from bound by the tensor pipe (8 rows: 16 FLOP
+// per weight byte), so what counts is that the operand needs no rearranging: a lane's 16 bytes of eight consecutive k are
+// used as the fragments of two products whose k order is permuted the same way in both operands, which a sum over k does
+// not see.  Gate and up weights come through a ring of bulk copies in shared memory, down weights straight from global
+// memory into registers.  Every result is summed in a fixed order, without atomics on floats.
+// 128 experts of 2048 x 768, top 8, bf16, all three launches: 190 us for 64 tokens (124 gate and up, 64 down; 96% of the
+// measured copy bandwidth), 91 for nine, 27 for one, of which 12 are its weights and the rest starts and routing.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -124,7 +126,10 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
       const int c = threadIdx.x >> 5;  // fragment component: expert g + 8 (c / 2), token 2 t4 + c % 2
       double v = 0.0;
 #pragma unroll
-      for (int i = 0; i < kRouteWarps; ++i) v += static_cast<double>(part[i][c][lane].x) + static_cast<double>(part[i][c][lane].y);
+      for (int i = 0; i < kRouteWarps; ++i) {
+        const float2 s = part[i][c][lane];
+        v += s.y == s.y ? static_cast<double>(s.x) + static_cast<double>(s.y) : static_cast<double>(s.x);  // infinite: no remainder
+      }
       const int e = e0 + g + 8 * (c >> 1);
       if (e < e_hi) cluster.map_shared_rank(logits, 2 * t4 + (c & 1))[e] = v + 0.0;  // -0 counts as +0
     }
@@ -198,9 +203,9 @@ struct Lists {
   int n_used, n_units, most;
 };
 
-__host__ __device__ constexpr int lists_bytes(int n, int E) { 
+__host__ __device__ constexpr int lists_bytes(int n, int E) {
   return (4 * 3 * 32 + 4 * E + 2 * (E + 1) * 2 + 2 * E + 2 * n + 127) / 128 * 128;
- }
+}
 
 __device__ __forceinline__ Lists build_lists(char* smem, const int* idx, int n, int E) {
   Lists L;
@@ -316,7 +321,7 @@ __device__ __forceinline__ Unit unit_at(const Lists& L, int unit) {
 // The weight stream.  An item is 16 weight rows of one unit, in two blocks of eight rows that lie one behind the other in
 // memory.  A ring of stages takes a block each (or a piece of at most kMaxPiece columns of it); one lane fills it with
 // bulk copies as far ahead as the ring is long, a whole block in a copy where it fits: a copy costs the engine about 90
-// cycles whatever its size, so that rows of 1.5 KB one by one would come at 4.8 TB/s and 12 KB blocks come at 6.7.
+// cycles whatever its size: rows of 1.5 KB one by one came at 4.8 TB/s, blocks of 16 to 32 KB come at 6.7 to 6.9.
 // Eight warps take a share of every piece's columns each; their sums meet in shared memory at the end of the item.
 // ---------------------------------------------------------------------------
 constexpr int kConsumers = 8;

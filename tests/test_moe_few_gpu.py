@@ -86,6 +86,24 @@ def test_ties_nan_repeated_and_missing_experts():
     assert ((out.double() - want).abs() <= bound + 2.0**-8 * want.abs()).all() and not out[2].any()
 
 
+@pytest.mark.parametrize("E,H", [(40, 64), (300, 520)])
+def test_infinite_logits(E, H):
+    """An expert with a logit of -inf is left out without spoiling its row; one of +inf comes first, and the weights are
+    those of the definition (inf - inf)."""
+    h, rw, *_ = make(3, E, 3, H, 8, device="cuda", dtype=BF)
+    h[:, 9] = torch.tensor([1.0, 2.0, 0.5], device="cuda")
+    rw[5, 9] = float("-inf")
+    for norm in (True, False):
+        w, idx = moe_few.route_few(h, rw, 3, norm)
+        w64, i64 = route64(h, rw, 3, norm)
+        assert torch.equal(idx.long(), i64) and not (idx == 5).any()
+        assert (w.double() - w64).abs().max() <= 2.0**-20
+    rw[7, 9] = float("inf")
+    w, idx = moe_few.route_few(h, rw, 3)
+    cw, cidx = moe_few.route_few(h.cpu(), rw.cpu(), 3)
+    assert (idx[:, 0] == 7).all() and torch.equal(idx.cpu(), cidx) and torch.equal(torch.isnan(w).cpu(), torch.isnan(cw))
+
+
 def test_capture_replays_on_new_routing():
     h, rw, wgu, wd = make(12, 32, 4, 128, 64, device="cuda", dtype=BF)
 
