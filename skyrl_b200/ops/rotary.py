@@ -203,6 +203,8 @@ def _launch_bwd(dy, x, q_norm, k_norm, pos, table, nq, nk, D, eps, interleaved, 
         # added in place where every wanted gradient has its fp32 buffer; a mix goes through fp32 zeros
         direct = all(g is not None and g.is_contiguous() and g.dtype == torch.float32
                      for g, on in ((mq, want_q), (mk, want_k)) if on)
+        if direct and want_q and want_k and abs(mq.data_ptr() - mk.data_ptr()) < 4 * D:
+            direct = False  # one weight for queries and keys: the kernel would add to its buffer twice at once
         mixed = not direct
         dqw, dkw = (mq, mk) if direct else (torch.zeros_like(w, dtype=torch.float32) if on else None
                                             for w, on in ((q_norm, want_q), (k_norm, want_k)))

@@ -143,6 +143,18 @@ def test_weight_gradients_go_to_main_grad_and_accumulate():
     assert torch.allclose(qw.main_grad, 1 + 2 * want[0], atol=1e-5) and torch.allclose(kw.main_grad, 2 * want[1], atol=1e-5)
 
 
+def test_one_weight_for_queries_and_keys():
+    g = torch.Generator().manual_seed(2)
+    x, w = torch.randn(6, 48, generator=g), torch.nn.Parameter(1 + 0.1 * torch.randn(16, generator=g))
+    pos, table = torch.arange(6, dtype=torch.int32), ew.build_rope_table(6, 16, 1e4, "cpu")
+    call = lambda: rotary.qk_norm_rope(x, w, w, pos, table, 1, 1, 16, 1e-6).square().sum().backward()  # noqa: E731
+    call()
+    want, w.grad = w.grad.clone(), None
+    w.main_grad = torch.zeros(16)
+    call()
+    assert w.grad is None and torch.allclose(w.main_grad, want, atol=1e-5)
+
+
 def test_cache_rows_partial_sums_and_empty_slots():
     g = torch.Generator().manual_seed(1)
     T, nq, nkv, D, bs = 9, 3, 2, 16, 4

@@ -193,6 +193,20 @@ def test_long_cache_offsets_pass_32_bits():
     assert not kc.any()
 
 
+def test_one_weight_for_queries_and_keys():
+    """Both gradients go to one buffer: to its fp32 main_grad and through the rows' type."""
+    T, nq, nkv, D = 2000, 4, 4, 64
+    x, dy, w, _, pos, table, *_ = make(T, nq, nkv, D, D, BF)
+    q, k = w.clone().requires_grad_(), w.clone().requires_grad_()
+    dq, dk = torch.autograd.grad(rotary.qk_norm_rope(x, q, k, pos, table, nq, nkv, D, 1e-6), (q, k), dy)
+    one = torch.nn.Parameter(w.clone())
+    one.main_grad = torch.zeros(D, device="cuda")
+    rotary.qk_norm_rope(x, one, one, pos, table, nq, nkv, D, 1e-6).backward(dy)
+    # the two sums are fp32 in the buffer and were rounded to bf16 above, half a step each
+    assert one.grad is None
+    assert ((one.main_grad - dq.float() - dk.float()).abs() <= 2.0**-8 * (dq.float().abs() + dk.float().abs()) + 2.0**-20).all()
+
+
 @pytest.mark.parametrize("D,R", [(64, 32), (24, 10)])
 def test_position_outside_the_table(D, R):
     x, dy, qw, kw, pos, table, *_ = make(6, 2, 1, D, R, BF, max_pos=16)
