@@ -126,7 +126,8 @@ struct Sum {
     lo += (hi - (s - b)) + (v - b);  // what the addition rounded away
     hi = s;
   }
-  __device__ __forceinline__ float get() const { return hi + lo; }
+  // an infinite sum has no finite remainder (inf - inf)
+  __device__ __forceinline__ float get() const { return lo == lo ? hi + lo : hi; }
 };
 
 // Sum over the 1 << lg consecutive lanes of a head.
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     long long slot = -1;
     if (!kBack && a.slots) slot = a.slots[t];
     char* piece = mine + stage * stage_bytes;
-    if (!mbar_wait(&bar[stage], parity, status, 0x4d10)) {
+    if (!__all_sync(0xffffffffu, mbar_wait(&bar[stage], parity, status, 0x4d10))) {  // the warp gives up as one
       ok = false;
       break;
     }

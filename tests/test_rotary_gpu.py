@@ -207,6 +207,19 @@ def test_one_weight_for_queries_and_keys():
     assert ((one.main_grad - dq.float() - dk.float()).abs() <= 2.0**-8 * (dq.float().abs() + dk.float().abs()) + 2.0**-20).all()
 
 
+@pytest.mark.parametrize("D", [64, 24])
+def test_infinite_partial_sums_stay_infinite(D):
+    x, _, _, _, pos, table, *_ = make(4, 2, 1, D, D, BF)
+    part = torch.stack([x.float(), torch.ones(4, 4 * D, device="cuda"), torch.zeros(4, 4 * D, device="cuda")])
+    part[1, 1, 3 * D + 2], part[1, 2, 3 * D + 5] = float("inf"), float("-inf")  # value heads
+    part[1, 3, 3 * D + 7], part[2, 3, 3 * D + 7] = float("inf"), float("-inf")
+    kc, vc = (torch.zeros(1, 4, 1, D, device="cuda", dtype=BF) for _ in range(2))
+    slots = torch.arange(4, device="cuda", dtype=torch.int32)
+    y = rotary.qk_rope_cache(part, pos, table, kc, vc, slots, 2, 1, D)
+    assert y[1, 3 * D + 2] == float("inf") and y[2, 3 * D + 5] == float("-inf") and torch.isnan(y[3, 3 * D + 7])
+    assert torch.isfinite(y).sum() == y.numel() - 3 and torch.equal(vc.view(4, D).view(torch.int16), y[:, 3 * D :].view(torch.int16))
+
+
 @pytest.mark.parametrize("D,R", [(64, 32), (24, 10)])
 def test_position_outside_the_table(D, R):
     x, dy, qw, kw, pos, table, *_ = make(6, 2, 1, D, R, BF, max_pos=16)
