@@ -29,8 +29,8 @@ __device__ __forceinline__ long long layout_block_sum(long long v, long long* re
 }
 
 __global__ void __launch_bounds__(kLayoutThreads)
-paged_layout_kernel(const int* tables, long long table_stride, int width, const int* starts, const int* lens, int B, int bs, int total, int* __restrict__ cu, int* __restrict__ pos,
-                    int* __restrict__ slots, int* __restrict__ whole) {
+paged_layout_kernel(const int* tables, long long table_stride, int width, const int* starts, const int* lens, int B, int bs,
+                    int total, int* __restrict__ cu, int* __restrict__ pos, int* __restrict__ slots, int* __restrict__ whole) {
   __shared__ long long red[kLayoutThreads / 32];
   pdl_launch_dependents();
   pdl_wait();

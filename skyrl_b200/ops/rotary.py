@@ -68,10 +68,34 @@ def _check_rows(x, what):
         raise ValueError(f"{what}: rows must be bf16, fp16 or fp32, got {x.dtype}")
 
 
+def _is_row_major(x: torch.Tensor) -> bool:
+    W = x.shape[1]
+    return (x.stride(1) == 1 or W == 1) and (x.stride(0) >= W or x.shape[0] <= 1)
+
+
 def _row_major(x: torch.Tensor) -> torch.Tensor:
     """Rows that the kernels can walk: unit stride inside a row, no two rows on the same memory."""
-    W = x.shape[1]
-    return x if (x.stride(1) == 1 or W == 1) and (x.stride(0) >= W or x.shape[0] <= 1) else x.contiguous()
+    return x if _is_row_major(x) else x.contiguous()
+
+
+def _share_memory(x: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether ``out`` overlaps ``x`` without being the same rows (columns of one buffer beside each other do not)."""
+    def end(t):
+        return t.data_ptr() + ((t.shape[-2] - 1) * t.stride(-2) + t.shape[-1]) * t.element_size()
+
+    if out.shape[0] == 0 or out.get_device() != x.get_device():
+        return False
+    if x.dim() == 3:
+        return x.data_ptr() < end(out) and out.data_ptr() < end(x[-1])
+    if out.data_ptr() == x.data_ptr():
+        return x.shape[0] > 1 and out.stride() != x.stride()
+    if not _is_row_major(x) or out.data_ptr() >= end(x) or x.data_ptr() >= end(out):  # the first: read from a copy
+        return False
+    if x.shape[0] == 1 or out.stride(0) != x.stride(0):
+        return True
+    W, step = x.shape[1], x.stride(0)
+    between = (out.data_ptr() - x.data_ptr()) // x.element_size() % step
+    return between < W or step - between < W
 
 
 # ----------------------------------------------------------------------------- PyTorch formulation
@@ -268,7 +292,7 @@ def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cac
     dt = k_cache.dtype
     if dt not in _DTYPE or v_cache.dtype != dt or x.dtype != (torch.float32 if partial else dt):
         raise ValueError(f"{what}: rows {x.dtype} and caches {dt}, {v_cache.dtype} do not go together")
-    if x.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, q_norm, k_norm)):
         raise ValueError(f"{what} has no gradient: use qk_norm_rope or rotary where one is needed")
     _check(x, pos, table, nq, nkv, head_dim, q_norm, k_norm, what)
     T, W = x.shape[-2:]
@@ -290,6 +314,8 @@ def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cac
     if out is not None and (out.shape != (T, W) or out.dtype != dt or out.get_device() != x.get_device() or out.stride(1) != 1
                             or (T > 1 and out.stride(0) < W)):
         raise ValueError(f"{what}: out must be [{T}, {W}] rows in the caches' type")
+    if out is not None and _share_memory(x, out):
+        raise ValueError(f"{what}: out lies on other elements of x (it may be x itself)")
     if not x.is_cuda:
         rows = x.double().sum(0).float().to(dt) if partial else x
         res = _fwd_ref(rows, q_norm, k_norm, pos, table, nq, nkv, head_dim, eps, interleaved, 1.0)
@@ -302,7 +328,5 @@ def qk_rope_cache(x: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, k_cac
         x = _row_major(x)
     if out is None:
         out = torch.empty((T, W), device=x.device, dtype=dt)
-    elif out.data_ptr() == x.data_ptr() and not partial and out.stride() != x.stride() and T > 1:
-        raise ValueError(f"{what}: out lies on x with other strides")
     return _launch_fwd(x, out, q_norm, k_norm, pos, table, nq, nkv, head_dim, float(eps), bool(interleaved), 1.0,
                        x.shape[0] if partial else 0, slots, k_cache, v_cache)

@@ -208,6 +208,31 @@ def test_refusals():
             rotary.qk_rope_cache(a["x"], pos, table, a["kc"], a["vc"], a["slots"], a["nq"], 1, 16, out=a["out"])
 
 
+def test_cache_rows_refuse_weights_with_gradients_and_overlapping_rows():
+    buf = torch.randn(8, 112)
+    x, pos, table = buf[:4, :48], torch.arange(4, dtype=torch.int32), ew.build_rope_table(8, 16, 1e4, "cpu")
+    kc, vc, slots, w = torch.zeros(2, 4, 1, 16), torch.zeros(2, 4, 1, 16), torch.arange(4, dtype=torch.int32), torch.ones(16)
+
+    def run(out, x=x, q_norm=None, k_norm=None):
+        return rotary.qk_rope_cache(x, pos, table, kc, vc, slots, 1, 1, 16, q_norm=q_norm, k_norm=k_norm, out=out)
+
+    for q, k in ((w.clone().requires_grad_(), w), (w, w.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="gradient"):
+            run(None, q_norm=q, k_norm=k)
+        with torch.no_grad():
+            run(None, q_norm=q, k_norm=k)
+    part = torch.randn(3, 4, 48)
+    for out in (buf[1:5, :48], buf[:4, 16:64], buf.view(-1)[: 4 * 56].view(4, 56)[:, :48]):
+        with pytest.raises(ValueError, match="lies on"):
+            run(out)
+    with pytest.raises(ValueError, match="lies on"):
+        run(part[1], x=part)
+    want = run(None)
+    for out in (buf[4:, :48], buf[:4, 48:96], buf[1:5, 64:]):  # other rows; columns beside
+        assert torch.equal(run(out), want)
+    assert torch.equal(run(x), want)
+
+
 # ----------------------------------------------------------------------------- paged layout
 def layout_oracle(tables, lens, starts, bs, total):
     cu, pos, slots, rows, whole = [0], [], [], [], 0
