@@ -12,7 +12,7 @@
 // not see.  Gate and up weights come through a ring of bulk copies in shared memory, down weights straight from global
 // memory into registers.  Every result is summed in a fixed order, without atomics on floats.
 // 128 experts of 2048 x 768, top 8, bf16, all three launches: 190 us for 64 tokens (124 gate and up, 64 down; 96% of the
-// measured copy bandwidth), 91 for nine, 27 for one, of which 12 are its weights and the rest starts and routing.
+// measured copy bandwidth), 91 for nine, 24 for one, of which 12 are its weights and the rest starts and routing.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -67,7 +67,7 @@ __device__ __forceinline__ int rank_of(const unsigned long long* key, int n, uns
   return before + __shfl_xor_sync(0xffffffffu, before, 1);
 }
 
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kRouteThreads, 2)
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kRouteThreads, 1)
 route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv_bfloat16* __restrict__ rw,
              const int* __restrict__ live, float* __restrict__ w, int* __restrict__ idx, int T, int E, int H, int k, int norm) {
   __shared__ float2 part[kRouteWarps][4][32];
@@ -91,7 +91,7 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
     const __nv_bfloat16* top = rw + static_cast<size_t>(min(e0 + g, e_hi - 1)) * H + 8 * t4;
     const __nv_bfloat16* low = rw + static_cast<size_t>(min(e0 + g + 8, e_hi - 1)) * H + 8 * t4;
     float hi[4] = {0.f, 0.f, 0.f, 0.f}, lo[4] = {0.f, 0.f, 0.f, 0.f};
-    constexpr int kUnroll = 4;
+    constexpr int kUnroll = 8;
     for (int s = s0; s < s1; s += kUnroll) {
       uint4 a[kUnroll], b[kUnroll], v[kUnroll];
 #pragma unroll
@@ -513,6 +513,7 @@ gate_up_kernel(const __nv_bfloat16* h, long long h_stride, const int* idx, const
   char* buf = smem + kRedBytes;
   ring_init(ring, s.stages);
   pdl_wait();
+  pdl_launch_dependents();
   const Lists L = build_lists(buf + static_cast<size_t>(s.stages) * 16 * s.piece, idx, n, E);
   const int tiles = (F + 7) >> 3;
   const long long items = static_cast<long long>(L.n_units) * tiles;
@@ -634,6 +635,21 @@ __device__ __forceinline__ void down_unit(const Lists& L, float* y, const __nv_b
     }
 }
 
+// The combination of a CTA's 16 columns from y [T * k][16]: slot by slot, so that the order is always the same.
+__device__ __forceinline__ void combine(const float* y, const int* idx, const float* w, __nv_bfloat16* out, int n0, int T, int k,
+                                        int E, int H) {
+  for (int i = threadIdx.x; i < T * 16; i += kDownThreads) {
+    const int t = i >> 4, c = i & 15;
+    if (n0 + c >= H) continue;
+    float v = 0.f;
+    for (int j = 0; j < k; ++j) {
+      const int e = idx[t * k + j];
+      if (e >= 0 && e < E) v = fmaf(w[t * k + j], y[(t * k + j) * 16 + c], v);
+    }
+    out[static_cast<size_t>(t) * H + n0 + c] = __float2bfloat16_rn(v);
+  }
+}
+
 __global__ void __launch_bounds__(kDownThreads, 1)
 down_kernel(const __nv_bfloat16* act, const int* __restrict__ idx, const float* w, const __nv_bfloat16* __restrict__ wd,
             __nv_bfloat16* __restrict__ out, int T, int k, int E, int H, int F) {
@@ -650,16 +666,110 @@ down_kernel(const __nv_bfloat16* act, const int* __restrict__ idx, const float* 
       down_unit<2>(L, y, act, wd, u, n0, H, F);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < T * 16; i += kDownThreads) {
-    const int t = i >> 4, c = i & 15;
-    if (n0 + c >= H) continue;
-    float v = 0.f;
-    for (int j = 0; j < k; ++j) {
-      const int e = idx[t * k + j];
-      if (e >= 0 && e < E) v = fmaf(w[t * k + j], y[(t * k + j) * 16 + c], v);
-    }
-    out[static_cast<size_t>(t) * H + n0 + c] = __float2bfloat16_rn(v);
+  combine(y, idx, w, out, n0, T, k, E, H);
+}
+
+// The same for so few entries that all weights a CTA needs fit into its shared memory at once (one token with eight experts
+// of width 768).  A CTA starts when the first kernel's CTA on its SM ends, fetches its weights (a unit's 16 rows lie one
+// behind the other: one bulk copy) while others of that kernel still run, and only then waits for the activations.  The
+// routing table is complete by then: the kernel before waits for it before it lets this one start.  Both expert kernels
+// for that token: 19.4 us, 22.9 with the kernel above in its place.
+constexpr int kOnceUnits = 32;
+
+template <int kNt>
+__device__ __forceinline__ void once_unit(const Lists& L, float* y, const char* wgt, const char* act, const Unit& u, int rows, int F) {
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  const char* top = wgt + static_cast<size_t>(min(g, rows - 1)) * 2 * F + 16 * t4;
+  const char* low = wgt + static_cast<size_t>(min(g + 8, rows - 1)) * 2 * F + 16 * t4;
+  const char* x[kNt];
+  float acc[kNt][4];
+#pragma unroll
+  for (int n = 0; n < kNt; ++n) {
+    const int r = u.r0 + n * 8 + g;
+    x[n] = r < u.r1 ? act + static_cast<size_t>(r) * 2 * F + 16 * t4 : nullptr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
   }
+  const int steps = (F - 8 * t4 + 31) >> 5, all = (F + 31) >> 5;  // of this lane; lane t4 = 0 has the most
+  const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+  for (int s = 0; s < all; ++s) {
+    const bool ok = s < steps;
+    const uint4 a = ok ? *reinterpret_cast<const uint4*>(top + s * 64) : z;
+    const uint4 b = ok ? *reinterpret_cast<const uint4*>(low + s * 64) : z;
+#pragma unroll
+    for (int n = 0; n < kNt; ++n) {
+      const uint4 v = ok && x[n] ? *reinterpret_cast<const uint4*>(x[n] + s * 64) : z;
+      mma_bf16(acc[n], a.x, b.x, a.y, b.y, v.x, v.y);
+      mma_bf16(acc[n], a.z, b.z, a.w, b.w, v.z, v.w);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kNt; ++n)
+#pragma unroll
+    for (int col = 0; col < 2; ++col) {
+      const int r = u.r0 + n * 8 + 2 * t4 + col;
+      if (r < u.r1) {
+        float* o = y + L.entry[r] * 16;
+        o[g] = acc[n][col];
+        o[g + 8] = acc[n][2 + col];
+      }
+    }
+}
+
+__host__ __device__ constexpr size_t once_bytes(int n, int F) { return static_cast<size_t>(n) * (34 * F + 64); }
+
+__global__ void __launch_bounds__(kDownThreads, 1)
+down_once_kernel(const __nv_bfloat16* act, const int* idx, const float* w, const __nv_bfloat16* __restrict__ wd, __nv_bfloat16* out,
+                 int T, int k, int E, int H, int F, int* status) {
+  extern __shared__ __align__(128) char smem[];
+  __shared__ uint64_t full[kOnceUnits];
+  const int n = T * k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kWarps = kDownThreads / 32;
+  char* wgt = smem;                                     // [units][16][F]
+  char* rows = smem + static_cast<size_t>(n) * 32 * F;  // [n][F], by place in the lists
+  float* y = reinterpret_cast<float*>(rows + static_cast<size_t>(n) * 2 * F);
+  if (threadIdx.x < n) mbar_init(&full[threadIdx.x], 1);
+  if (threadIdx.x < 32) fence_mbar_init();
+  const Lists L = build_lists(smem + once_bytes(n, F), idx, n, E);  // its barriers also order the lines above
+  const int n0 = blockIdx.x * 16, n_rows = min(16, H - n0);
+  if (lane == 0) {
+    fence_proxy_async_global();
+    for (int i = warp; i < L.n_units; i += kWarps) {
+      const uint32_t bytes = 2u * F * n_rows;
+      mbar_arrive_expect_tx(&full[i], bytes);
+      bulk_load(wgt + static_cast<size_t>(i) * 32 * F, wd + (static_cast<size_t>(unit_at(L, i).e) * H + n0) * F, bytes, &full[i]);
+    }
+  }
+  __syncwarp();
+  pdl_wait();
+  for (int i = warp; i < L.n_units; i += kWarps) {
+    const Unit u = unit_at(L, i);
+    for (int r = u.r0; r < u.r1; ++r) {
+      const uint4* from = reinterpret_cast<const uint4*>(act + static_cast<size_t>(L.entry[r]) * F);
+      uint4* to = reinterpret_cast<uint4*>(rows + static_cast<size_t>(r) * 2 * F);
+#pragma unroll 4
+      for (int c = lane; c < F / 8; c += 32) to[c] = from[c];
+    }
+  }
+  __syncwarp();
+  for (int i = warp; i < L.n_units; i += kWarps) {
+    if (!mbar_wait(&full[i], 0, status, 0x4d04)) {  // the copy still lands before the buffer is given back
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(&full[i], 0))
+        if (globaltimer_ns() - t0 > kWaitTimeoutNs / 100) break;
+      continue;
+    }
+    const Unit u = unit_at(L, i);
+    const char* mine = wgt + static_cast<size_t>(i) * 32 * F;
+    if (u.r1 - u.r0 <= 8)
+      once_unit<1>(L, y, mine, rows, u, n_rows, F);
+    else
+      once_unit<2>(L, y, mine, rows, u, n_rows, F);
+  }
+  __syncthreads();
+  combine(y, idx, w, out, n0, T, k, E, H);
 }
 
 // Stages of eight rows of K columns in `room` bytes.  A row of more than kMaxPiece columns comes in equal pieces.
@@ -700,6 +810,19 @@ cudaError_t launch_down(const void* act, const int* idx, const float* w, const v
                                                          static_cast<const __nv_bfloat16*>(wd), static_cast<__nv_bfloat16*>(out), T, k,
                                                          E, H, F);
   return cudaGetLastError();
+}
+
+cudaError_t launch_down_once(const void* act, const int* idx, const float* w, const void* wd, void* out, int T, int k, int E, int H,
+                             int F, size_t smem, size_t smem_most, int* status, cudaStream_t st) {
+  static bool attr_dev[64] = {};
+  bool& attr = attr_dev[device_index()];
+  if (!attr) {
+    const cudaError_t e = cudaFuncSetAttribute(down_once_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_most));
+    if (e != cudaSuccess) return e;
+    attr = true;
+  }
+  return launch_pdl(down_once_kernel, dim3((H + 15) / 16), dim3(kDownThreads), smem, st, static_cast<const __nv_bfloat16*>(act), idx, w,
+                    static_cast<const __nv_bfloat16*>(wd), static_cast<__nv_bfloat16*>(out), T, k, E, H, F, status);
 }
 
 }  // namespace mf
@@ -743,7 +866,11 @@ int sb_moe_few_experts(const void* h, long long h_stride, const float* w, const 
   cudaError_t e = (gu.piece <= 1024 ? sb::mf::launch_gate_up<4> : sb::mf::launch_gate_up<8>)(h, h_stride, idx, wgu, act, T, k, E, H, F, gu,
                                                                                               smem_gu, most, status, st);
   if (e != cudaSuccess) return SB_ERR_CUDA;
-  e = sb::mf::launch_down(act, idx, w, wd, out, T, k, E, H, F, sizeof(float) * 16 * static_cast<size_t>(n) + lists, most, st);
+  const size_t once = sb::mf::once_bytes(n, F) + lists;
+  if (n <= sb::mf::kOnceUnits && once <= most)
+    e = sb::mf::launch_down_once(act, idx, w, wd, out, T, k, E, H, F, once, most, status, st);
+  else
+    e = sb::mf::launch_down(act, idx, w, wd, out, T, k, E, H, F, sizeof(float) * 16 * static_cast<size_t>(n) + lists, most, st);
   return e == cudaSuccess ? SB_OK : SB_ERR_CUDA;
 }
 
