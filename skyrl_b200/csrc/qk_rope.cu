@@ -441,7 +441,29 @@ __device__ __forceinline__ void put4(__half* p, const float (&e)[4]) {
 }
 __device__ __forceinline__ void put4(float* p, const float (&e)[4]) { *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(e); }
 
-// The first (a) and second (b) members of a lane's four pairs, two at a time; its elements start at lo and hi.
+// Two neighbouring elements.
+__device__ __forceinline__ f2 get2(const __nv_bfloat16* p) {
+  const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+  return pack2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ f2 get2(const __half* p) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(p));
+  return pack2(v.x, v.y);
+}
+__device__ __forceinline__ f2 get2(const float* p) { return *reinterpret_cast<const f2*>(p); }
+__device__ __forceinline__ void put2(__nv_bfloat16* p, f2 v) {
+  float x, y;
+  unpack2(v, x, y);
+  *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(x, y);
+}
+__device__ __forceinline__ void put2(__half* p, f2 v) {
+  float x, y;
+  unpack2(v, x, y);
+  *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x, y);
+}
+__device__ __forceinline__ void put2(float* p, f2 v) { *reinterpret_cast<f2*>(p) = v; }
+
+// The first (a) and second (b) members of a lane's four pairs, two at a time.
 struct Pairs {
   f2 a[2], b[2];
 };
@@ -471,22 +493,31 @@ __device__ __forceinline__ void put8(T* p, const float (&l)[4], const float (&r)
     put4(p + 4, r);
   }
 }
-template <typename T, bool kInter>
-__device__ __forceinline__ Pairs get_pairs(const T* p, int lo, int hi) {
+// Where a lane's elements lie in a head: its four first members, or its first two pairs' and its last two pairs'.
+struct Spot {
+  int lo, hi;    // first and second members of pairs 0 and 1; without kFine of all four
+  int lo2, hi2;  // of pairs 2 and 3
+};
+template <typename T, bool kInter, bool kFine>
+__device__ __forceinline__ Pairs get_pairs(const T* p, const Spot& at) {
+  Pairs v;
+  if (kFine && !kInter) {
+    v.a[0] = get2(p + at.lo);
+    v.b[0] = get2(p + at.hi);
+    v.a[1] = get2(p + at.lo2);
+    v.b[1] = get2(p + at.hi2);
+    return v;
+  }
   float l[4], r[4];
   if (kInter) {
-    get8(p + lo, l, r);
-  } else {
-    get4(p + lo, l);
-    get4(p + hi, r);
-  }
-  Pairs v;
-  if (kInter) {
+    get8(p + at.lo, l, r);
     v.a[0] = pack2(l[0], l[2]);
     v.b[0] = pack2(l[1], l[3]);
     v.a[1] = pack2(r[0], r[2]);
     v.b[1] = pack2(r[1], r[3]);
   } else {
+    get4(p + at.lo, l);
+    get4(p + at.hi, r);
     v.a[0] = pack2(l[0], l[1]);
     v.a[1] = pack2(l[2], l[3]);
     v.b[0] = pack2(r[0], r[1]);
@@ -494,25 +525,29 @@ __device__ __forceinline__ Pairs get_pairs(const T* p, int lo, int hi) {
   }
   return v;
 }
-template <typename T, bool kInter>
-__device__ __forceinline__ void put_pairs(T* p, int lo, int hi, const Pairs& v) {
+template <typename T, bool kInter, bool kFine>
+__device__ __forceinline__ void put_pairs(T* p, const Spot& at, const Pairs& v) {
+  if (kFine && !kInter) {
+    put2(p + at.lo, v.a[0]);
+    put2(p + at.hi, v.b[0]);
+    put2(p + at.lo2, v.a[1]);
+    put2(p + at.hi2, v.b[1]);
+    return;
+  }
   float l[4], r[4];
   if (kInter) {
     unpack2(v.a[0], l[0], l[2]);
     unpack2(v.b[0], l[1], l[3]);
     unpack2(v.a[1], r[0], r[2]);
     unpack2(v.b[1], r[1], r[3]);
+    put8(p + at.lo, l, r);
   } else {
     unpack2(v.a[0], l[0], l[1]);
     unpack2(v.a[1], l[2], l[3]);
     unpack2(v.b[0], r[0], r[1]);
     unpack2(v.b[1], r[2], r[3]);
-  }
-  if (kInter) {
-    put8(p + lo, l, r);
-  } else {
-    put4(p + lo, l);
-    put4(p + hi, r);
+    put4(p + at.lo, l);
+    put4(p + at.hi, r);
   }
 }
 
@@ -530,7 +565,8 @@ constexpr int kRowWarps = 16;
 
 enum Mode { kRotate, kNormRotate, kNormBack };
 
-template <typename T, bool kInter, Mode kMode>
+// kFine: the rotated width is a multiple of 4, not of 8, so that a lane may own two pairs that rotate and two that do not.
+template <typename T, bool kInter, bool kFine, Mode kMode>
 __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, int piece_bytes, int* status) {
   constexpr bool kBack = kMode == kNormBack;
   extern __shared__ __align__(128) char smem[];
@@ -549,7 +585,17 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
   const int hpw = 32 >> a.log_group;
   const int c = lane & ((1 << a.log_group) - 1), sub = lane >> a.log_group;
   const bool live = c * 8 < a.D, rot = c * 8 < a.R;  // a lane without elements goes along with the first one's
-  const int lo = !live ? 0 : kInter || !rot ? 8 * c : 4 * c, hi = kInter || !rot ? lo + 4 : (a.R >> 1) + 4 * c;
+  const int half = a.R >> 1;
+  const bool rot2 = kFine ? 4 * c + 2 < half : rot;  // pairs 2 and 3
+  Spot at;
+  at.lo = !live ? 0 : kInter || !rot ? 8 * c : 4 * c;
+  if (kFine) {
+    at.hi = rot && live ? half + 4 * c : at.lo + 2;
+    at.lo2 = !live ? 4 : rot2 ? 4 * c + 2 : 8 * c + 4;
+    at.hi2 = rot2 && live ? half + 4 * c + 2 : at.lo2 + 2;
+  } else {
+    at.hi = kInter || !rot ? at.lo + 4 : half + 4 * c;
+  }
   const int turned = a.nq + a.nk;
   const int head_bytes = a.D * static_cast<int>(sizeof(T));
   const int block_heads = piece_bytes / head_bytes;
@@ -577,14 +623,14 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     if (kBack && nx > 0)
       bulk_load(dst + piece_bytes, static_cast<const T*>(a.x) + static_cast<size_t>(p.t) * a.x_stride + h0 * a.D, nx, &bar[stage]);
   };
-  Place now, ahead, at;  // the piece in work, the one to be loaded next, the one whose position is read next
+  Place now, ahead, next;  // the piece in work, the one to be loaded next, the one whose position is read next
   now.t = first / a.blocks_per_row;
   now.blk = first - now.t * a.blocks_per_row;
-  ahead = at = now;
-  const int p_first = count > 0 ? a.pos[at.t] : 0;
-  advance(at);
-  int p_next = count > 1 ? a.pos[at.t] : 0;
-  advance(at);
+  ahead = next = now;
+  const int p_first = count > 0 ? a.pos[next.t] : 0;
+  advance(next);
+  int p_next = count > 1 ? a.pos[next.t] : 0;
+  advance(next);
   for (int i = 0; i < kStages - 1; ++i) {
     if (lane == 0 && i < count) fill(ahead, i);
     advance(ahead);
@@ -595,12 +641,24 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     if (!rot) return;
     if (p < 0 || p >= a.max_pos) {
       const float nan = __int_as_float(0x7fffffff);
-      cos_next = sin_next = make_float4(nan, nan, nan, nan);
+      cos_next = rot2 ? make_float4(nan, nan, nan, nan) : make_float4(nan, nan, 1.f, 1.f);
+      sin_next = rot2 ? make_float4(nan, nan, nan, nan) : make_float4(nan, nan, 0.f, 0.f);
       return;
     }
     const float* t = a.table + static_cast<size_t>(p) * a.R + 4 * c;
-    cos_next = __ldg(reinterpret_cast<const float4*>(t));
-    sin_next = __ldg(reinterpret_cast<const float4*>(t + (a.R >> 1)));
+    if (kFine) {
+      const float2 c0 = __ldg(reinterpret_cast<const float2*>(t)), s0 = __ldg(reinterpret_cast<const float2*>(t + half));
+      float2 c1 = make_float2(1.f, 1.f), s1 = make_float2(0.f, 0.f);
+      if (rot2) {
+        c1 = __ldg(reinterpret_cast<const float2*>(t + 2));
+        s1 = __ldg(reinterpret_cast<const float2*>(t + half + 2));
+      }
+      cos_next = make_float4(c0.x, c0.y, c1.x, c1.y);
+      sin_next = make_float4(s0.x, s0.y, s1.x, s1.y);
+    } else {
+      cos_next = __ldg(reinterpret_cast<const float4*>(t));
+      sin_next = __ldg(reinterpret_cast<const float4*>(t + half));
+    }
   };
   if (count > 0) angles(p_first);
 
@@ -617,8 +675,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     const f2 ss[2] = {pack2(sin_next.x * sg, sin_next.y * sg), pack2(sin_next.z * sg, sin_next.w * sg)};
     const f2 ns[2] = {pack2(sin_next.x * -sg, sin_next.y * -sg), pack2(sin_next.z * -sg, sin_next.w * -sg)};
     if (i + 1 < count) angles(p_next);
-    if (i + 2 < count) p_next = a.pos[at.t];
-    advance(at);
+    if (i + 2 < count) p_next = a.pos[next.t];
+    advance(next);
     const int t = now.t, h0 = now.blk * block_heads, h1 = min(a.heads, h0 + block_heads);
     advance(now);
     long long slot = -1;
@@ -631,7 +689,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     auto heads = [&](int from, int to, const T* w, f2 (&acc)[4]) {
       if (from >= to) return;
       Pairs wt, ca, sa;
-      if (kMode != kRotate) wt = get_pairs<T, kInter>(w, lo, hi);
+      if (kMode != kRotate) wt = get_pairs<T, kInter, kFine>(w, at);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         ca.a[j] = kMode == kNormRotate ? mul2(cc[j], wt.a[j]) : cc[j];
@@ -643,8 +701,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
       for (int h = from + sub; h - sub < to; h += hpw) {
         T* row = base + min(h, to - 1) * a.D;  // a lane behind the last head goes along with the last one's
         const bool on = live && h < to;
-        Pairs v = get_pairs<T, kInter>(row, lo, hi), x;
-        if (kBack) x = get_pairs<T, kInter>(row + piece_bytes / static_cast<int>(sizeof(T)), lo, hi);
+        Pairs v = get_pairs<T, kInter, kFine>(row, at), x;
+        if (kBack) x = get_pairs<T, kInter, kFine>(row + piece_bytes / static_cast<int>(sizeof(T)), at);
         float r = 1.f, m = 0.f;
         if (kMode != kRotate) {
           const Pairs& y = kBack ? x : v;
@@ -692,13 +750,14 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
         } else {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
+            if (kFine && kMode == kRotate && j == 1 && !rot2) continue;  // not times 1 plus 0: there may be infinities
             const f2 va = fma2(v.b[j], sa.b[j], mul2(v.a[j], ca.a[j]));
             const f2 vb = fma2(v.a[j], sa.a[j], mul2(v.b[j], ca.b[j]));
             v.a[j] = kMode == kNormRotate ? mul2(va, r2) : va;
             v.b[j] = kMode == kNormRotate ? mul2(vb, r2) : vb;
           }
         }
-        if (on && (kMode != kRotate || rot)) put_pairs<T, kInter>(row, lo, hi, v);
+        if (on && (kMode != kRotate || rot)) put_pairs<T, kInter, kFine>(row, at, v);
       }
     };
     heads(h0, min(h1, a.nq), static_cast<const T*>(a.qw), acc_q);
@@ -766,8 +825,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     float* s = sdw + warp * 2 * a.D;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      // pair j: interleaved pairs 0, 1 lie at lo, pairs 2, 3 at hi
-      const int ea = kInter ? (j < 2 ? lo : hi) + 2 * (j & 1) : lo + j, eb = kInter ? ea + 1 : hi + j;
+      // pair j: interleaved pairs 0, 1 lie at lo, pairs 2, 3 behind them
+      const int first_at = kFine && j > 1 ? at.lo2 + j - 2 : at.lo + j, second_at = kFine && j > 1 ? at.hi2 + j - 2 : at.hi + j;
+      const int ea = kInter ? at.lo + 2 * j : first_at, eb = kInter ? ea + 1 : second_at;
       s[ea] = aq[j];
       s[eb] = aq[4 + j];
       s[a.D + ea] = ak[j];
@@ -950,11 +1010,13 @@ reduce_dw_kernel(const float* part, int rows, int D, void* dq, void* dk, int acc
     static_cast<T*>(base)[e] = from_f<T>(v);
 }
 
-bool vectorised(const Args& a, size_t elt, int unit) {
+// Whether rows, weights, tables and caches can be read 16 bytes at a time by lanes that own `unit` elements of a head and
+// `rot_unit` of its rotated part.
+bool vectorised(const Args& a, size_t elt, int unit, int rot_unit) {
   const auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const long long per = 16 / static_cast<long long>(elt);
   const bool strides = a.n_part ? (a.src_stride % 4 == 0 && a.part_stride % 4 == 0) : a.src_stride % per == 0;
-  return a.D % unit == 0 && a.R % unit == 0 && strides && a.x_stride % per == 0 && a.dst_stride % per == 0 && al(a.src) &&
+  return a.D % unit == 0 && a.R % rot_unit == 0 && strides && a.x_stride % per == 0 && a.dst_stride % per == 0 && al(a.src) &&
          al(a.x) && al(a.dst) && al(a.qw) && al(a.kw) && al(a.table) && al(a.kc) && al(a.vc);
 }
 
@@ -967,8 +1029,8 @@ int log2_ceil(int v) {
 // The row pipeline: heads of a piece so that a CTA's buffers fill at most kRowSmem.
 constexpr int kRowSmem = 200 * 1024;
 
-template <typename T, bool kInter, Mode kMode>
-cudaError_t launch_rows(Args a, int ctas, cudaStream_t st) {
+template <typename T, bool kInter, bool kFine, Mode kMode>
+cudaError_t launch_rows_as(Args a, int ctas, cudaStream_t st) {
   const int head = a.D * static_cast<int>(sizeof(T)), per_head = kRowWarps * kStages * head * (kMode == kNormBack ? 2 : 1);
   int block = kRowSmem / per_head;  // as large as the buffers allow, and alike
   a.blocks_per_row = (a.heads + block - 1) / block;
@@ -979,30 +1041,40 @@ cudaError_t launch_rows(Args a, int ctas, cudaStream_t st) {
   static bool attr_dev[64] = {};
   bool& attr = attr_dev[device_index()];
   if (!attr) {
-    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, kInter, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
+    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, kInter, kFine, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
     if (e != cudaSuccess) return e;
     attr = true;
   }
   int* status = device_status_ptr();
   if (!status) return cudaErrorUnknown;
   a.log_group = log2_ceil(a.D / 8);
-  return launch_pdl(rows_kernel<T, kInter, kMode>, dim3(ctas), dim3(kRowWarps * 32), smem, st, a, block * head, status);
+  return launch_pdl(rows_kernel<T, kInter, kFine, kMode>, dim3(ctas), dim3(kRowWarps * 32), smem, st, a, block * head, status);
+}
+
+template <typename T, bool kInter, Mode kMode>
+cudaError_t launch_rows(const Args& a, int ctas, cudaStream_t st) {
+  return a.R % 8 ? launch_rows_as<T, kInter, true, kMode>(a, ctas, st) : launch_rows_as<T, kInter, false, kMode>(a, ctas, st);
 }
 
 // From how many bytes of rows on the pipeline is taken.  Below, its start (4 us against 2) costs more than it gains, and
 // rows that lie in L2 come fast enough through plain loads.  bf16, 40 heads of 128, plain kernel / pipeline in us: forward
 // of 23 MB 12.1 / 13.5, of 47 MB 28.3 / 23.5, of 160 MB 89.7 / 60.0; backward of 0.6 MB 6.2 / 6.8, of 1.5 MB 8.7 / 7.0, of
-// 160 MB 144 / 90.
+// 160 MB 144 / 90.  Head sizes and widths that would go element by element otherwise, where the number of elements counts:
+// 8 + 2 + 2 heads of 80, 40 rotated, element by element / pipeline: forward of 0.5 M elements 4.1 / 4.8, of 1 M 6.3 / 4.9,
+// of 16 M 79 / 20; backward of 0.25 M 7.8 / 8.5, of 0.5 M 10.3 / 8.7, of 16 M 146 / 30.
 constexpr long long kForwardFrom = 28LL << 20, kBackwardFrom = 640LL << 10;
-bool row_pipeline(const Args& a, size_t elt, long long from) {
-  return a.D <= 256 && vectorised(a, elt, 8) && static_cast<long long>(a.T) * a.heads * a.D * static_cast<long long>(elt) > from;
+constexpr long long kForwardFromElements = 800LL << 10, kBackwardFromElements = 350LL << 10;
+bool row_pipeline(const Args& a, size_t elt, long long from, long long from_elements) {
+  if (a.D > 256 || !vectorised(a, elt, 8, 4)) return false;
+  const long long elements = static_cast<long long>(a.T) * a.heads * a.D;
+  return vectorised(a, elt, 16, 16) ? elements * static_cast<long long>(elt) > from : elements > from_elements;
 }
 
 template <typename T, bool kInter, bool kNorm, bool kPart>
 cudaError_t launch_fwd(Args a, cudaStream_t st) {
-  if (!kPart && row_pipeline(a, sizeof(T), kForwardFrom))
+  if (!kPart && row_pipeline(a, sizeof(T), kForwardFrom, kForwardFromElements))
     return launch_rows<T, kInter, kNorm ? kNormRotate : kRotate>(a, sm_count(), st);
-  if (!vectorised(a, sizeof(T), 16)) {
+  if (!vectorised(a, sizeof(T), 16, 16)) {
     const long long ctas = (static_cast<long long>(a.T) * a.heads + kWarps - 1) / kWarps;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_pdl(fwd_any_kernel<T, kInter, kNorm, kPart>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0, st, a);
@@ -1035,11 +1107,11 @@ int bwd_ctas(long long items) {
 template <typename T, bool kInter>
 cudaError_t launch_bwd(Args a, int& ctas, cudaStream_t st) {
   const size_t smem = sizeof(float) * kWarps * 2 * a.D;  // at most 32 KB (D <= 512)
-  if (row_pipeline(a, sizeof(T), kBackwardFrom)) {
+  if (row_pipeline(a, sizeof(T), kBackwardFrom, kBackwardFromElements)) {
     if (ctas > sm_count()) ctas = sm_count();
     return launch_rows<T, kInter, kNormBack>(a, ctas, st);
   }
-  if (!vectorised(a, sizeof(T), 16))
+  if (!vectorised(a, sizeof(T), 16, 16))
     return launch_pdl(bwd_any_kernel<T, kInter>, dim3(ctas), dim3(kThreads), smem, st, a);
   a.log_group = log2_ceil(a.D / 16);
   const int hpw = 32 >> a.log_group;

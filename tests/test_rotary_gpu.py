@@ -65,6 +65,9 @@ SIZES = [  # T, nq, nkv, D, R, interleaved, dtype, layout, scaling
     (12000, 10, 3, 80, 80, False, HF, "strided", "none"), (10000, 8, 4, 96, 24, False, BF, "plain", "llama3"),
     (4000, 8, 4, 256, 256, True, FP, "plain", "none"), (700, 4, 2, 80, 40, True, BF, "strided", "none"),
     (4001, 2, 1, 24, 8, False, FP, "plain", "none"), (801, 5, 3, 512, 64, False, HF, "plain", "none"),
+    (3000, 8, 2, 80, 20, False, BF, "plain", "none"), (2000, 5, 1, 80, 20, True, HF, "plain", "yarn"),
+    (1500, 4, 4, 96, 92, False, FP, "strided", "none"), (2500, 3, 1, 8, 4, False, BF, "plain", "none"),
+    (3001, 6, 2, 72, 36, False, HF, "plain", "linear"), (1999, 2, 2, 256, 12, True, BF, "plain", "none"),
 ]
 
 
@@ -230,6 +233,16 @@ def test_position_outside_the_table(D, R):
     for t in (y, d):
         nan = torch.isnan(t.view(6, 4, D))
         assert nan[[1, 4], :3, :R].all() and not nan[[1, 4], :3, R:].any() and not nan[:, 3].any() and not nan[[0, 2, 3, 5]].any()
+
+
+@pytest.mark.parametrize("T,D,R,inter", [(4, 40, 12, False), (9000, 40, 12, False), (9000, 40, 12, True), (9000, 64, 32, False)])
+def test_infinities_behind_the_rotated_part_stay_where_they_are(T, D, R, inter):
+    x, _, _, _, pos, table, *_ = make(T, 3, 1, D, R, BF)
+    at = torch.zeros_like(x, dtype=torch.bool).view(T, 5, D)
+    at[::2, :4, R], at[1::2, :4, R + 3] = True, True
+    x.view(T, 5, D)[at] = float("inf")
+    y = rotary.rotary(x, pos, table, 4, D, interleaved=inter)
+    assert torch.equal(y.view(T, 5, D)[..., R:], x.view(T, 5, D)[..., R:]) and torch.isfinite(y.view(T, 5, D)[..., :R]).all()
 
 
 def test_empty_batch_and_infinities_pass_through():
