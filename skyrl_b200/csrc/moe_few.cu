@@ -39,8 +39,10 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 // ---------------------------------------------------------------------------
 // Router.  A cluster of eight CTAs takes eight tokens and an eighth of the experts each, 16 experts at a time; the CTA's
 // warps split the columns, and the logits of token i meet in CTA i's shared memory.  Products of bf16 are exact in the
-// matrix unit; its fp32 sums are taken out every 32 columns and carried on in two fp32 words, so that experts whose
-// logits lie next to one another are ordered by the values and not by the rounding of a long sum.
+// matrix unit; its fp32 sums are taken out every 32 columns and carried on in two fp32 words, and where the order still
+// hangs on their error (one row in 700 at 128 experts) the logits in question are summed again in fp64: experts are ordered
+// by the values, equal ones by their number.  128 experts, rows of 2048: 4.8 us for one token, 5.4 for 64, of which 0.3 are
+// that check; a row with logits in question takes 3 to 4 more.
 // The k largest are found by rank, the number of experts that come before one: all are compared with one another at once,
 // where k rounds of a maximum would wait for one another.  Beyond kRankGroup experts, passes over groups leave k
 // candidates each, and a last pass ranks those.
@@ -49,6 +51,11 @@ constexpr int kCluster = 8;  // CTAs, and tokens
 constexpr int kRouteThreads = 256;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRankGroup = 128;  // entries ranked in a pass, two lanes each
+// Logits that lie closer than this share of the largest sum of magnitudes are compared in fp64.  A product of 16 columns
+// has 17 addends, each cut off at 2^-24 of the largest, which is at most about a third of their sum in rows of a model:
+// twice 17/3 * 2^-24 for two logits, just under 2^-20.
+constexpr double kLogitError = 1.0 / (1 << 20);
+constexpr int kExactBatch = 4;
 
 // Order-preserving key of a logit, unique: the lowest ten bits hold the expert, the lower one first among equals.  A NaN
 // comes last.
@@ -58,6 +65,17 @@ __device__ __forceinline__ unsigned long long logit_key(double v, int e) {
   return (k & ~1023ull) | static_cast<unsigned long long>(1023 - e);
 }
 __device__ __forceinline__ int key_expert(unsigned long long k) { return 1023 - static_cast<int>(k & 1023); }
+
+// z + the products of eight bf16 pairs, in fp64
+__device__ __forceinline__ double dot8(const uint4& a, const uint4& b, double z) {
+  const uint32_t p[4] = {a.x, a.y, a.z, a.w}, q[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    z = fma(static_cast<double>(__uint_as_float(p[j] << 16)), static_cast<double>(__uint_as_float(q[j] << 16)), z);
+    z = fma(static_cast<double>(__uint_as_float(p[j] & 0xffff0000u)), static_cast<double>(__uint_as_float(q[j] & 0xffff0000u)), z);
+  }
+  return z;
+}
 
 // Entries of key[0..n) above `mine`, counted by two neighbouring lanes.
 __device__ __forceinline__ int rank_of(const unsigned long long* key, int n, unsigned long long mine) {
@@ -71,9 +89,13 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kRouteThreads
 route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv_bfloat16* __restrict__ rw,
              const int* __restrict__ live, float* __restrict__ w, int* __restrict__ idx, int T, int E, int H, int k, int norm) {
   __shared__ float2 part[kRouteWarps][4][32];
+  __shared__ float part_mag[kRouteWarps][4][32], warp_mag[kRouteWarps];
   __shared__ unsigned long long key[kMaxExperts], cand[kRankGroup];
-  __shared__ int n_cand, chosen[kMaxTopK];
+  __shared__ int n_cand, n_close, chosen[kMaxTopK];
+  __shared__ unsigned short near[kMaxExperts];
+  __shared__ double exact_part[kExactBatch][kRouteWarps];
   extern __shared__ double logits[];  // [E], of token t0 + rank
+  float* mags = reinterpret_cast<float*>(logits + E);  // [E] sums of the products' magnitudes
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -90,7 +112,7 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
   for (int e0 = rank * per; e0 < e_hi; e0 += 16) {
     const __nv_bfloat16* top = rw + static_cast<size_t>(min(e0 + g, e_hi - 1)) * H + 8 * t4;
     const __nv_bfloat16* low = rw + static_cast<size_t>(min(e0 + g + 8, e_hi - 1)) * H + 8 * t4;
-    float hi[4] = {0.f, 0.f, 0.f, 0.f}, lo[4] = {0.f, 0.f, 0.f, 0.f};
+    float hi[4] = {0.f, 0.f, 0.f, 0.f}, lo[4] = {0.f, 0.f, 0.f, 0.f}, mag[4] = {0.f, 0.f, 0.f, 0.f};
     constexpr int kUnroll = 8;
     for (int s = s0; s < s1; s += kUnroll) {
       uint4 a[kUnroll], b[kUnroll], v[kUnroll];
@@ -108,6 +130,9 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
         float d[4] = {0.f, 0.f, 0.f, 0.f};
         mma_bf16(d, a[j].x, b[j].x, a[j].y, b[j].y, v[j].x, v[j].y);
         mma_bf16(d, a[j].z, b[j].z, a[j].w, b[j].w, v[j].z, v[j].w);
+        constexpr uint32_t kAbs = 0x7fff7fffu;
+        mma_bf16(mag, a[j].x & kAbs, b[j].x & kAbs, a[j].y & kAbs, b[j].y & kAbs, v[j].x & kAbs, v[j].y & kAbs);
+        mma_bf16(mag, a[j].z & kAbs, b[j].z & kAbs, a[j].w & kAbs, b[j].w & kAbs, v[j].z & kAbs, v[j].w & kAbs);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const float sum = hi[c] + d[c], back = sum - hi[c];
@@ -118,20 +143,28 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
     }
     if (waited) __syncthreads();  // the sums of the 16 experts before have been read
 #pragma unroll
-    for (int c = 0; c < 4; ++c) part[warp][c][lane] = make_float2(hi[c], lo[c]);
+    for (int c = 0; c < 4; ++c) {
+      part[warp][c][lane] = make_float2(hi[c], lo[c]);
+      part_mag[warp][c][lane] = mag[c];
+    }
     __syncthreads();
     if (!waited) cluster.barrier_wait();  // every CTA of the cluster runs before its shared memory is written
     waited = true;
     if (threadIdx.x < 128) {
       const int c = threadIdx.x >> 5;  // fragment component: expert g + 8 (c / 2), token 2 t4 + c % 2
       double v = 0.0;
+      float m = 0.f;
 #pragma unroll
       for (int i = 0; i < kRouteWarps; ++i) {
         const float2 s = part[i][c][lane];
         v += s.y == s.y ? static_cast<double>(s.x) + static_cast<double>(s.y) : static_cast<double>(s.x);  // infinite: no remainder
+        m += part_mag[i][c][lane];
       }
-      const int e = e0 + g + 8 * (c >> 1);
-      if (e < e_hi) cluster.map_shared_rank(logits, 2 * t4 + (c & 1))[e] = v + 0.0;  // -0 counts as +0
+      const int e = e0 + g + 8 * (c >> 1), to = 2 * t4 + (c & 1);
+      if (e < e_hi) {
+        cluster.map_shared_rank(logits, to)[e] = v + 0.0;  // -0 counts as +0
+        cluster.map_shared_rank(mags, to)[e] = m;
+      }
     }
   }
   if (!waited) cluster.barrier_wait();
@@ -146,43 +179,109 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
     return;
   }
   int bad = 0;
+  float top_mag = 0.f;
   for (int e = threadIdx.x; e < E; e += kRouteThreads) {
     const double v = logits[e];
     bad |= v != v;
     key[e] = logit_key(v, e);
+    top_mag = fmaxf(top_mag, mags[e]);
   }
+  top_mag = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_mag)));  // none is negative
+  if (lane == 0) warp_mag[warp] = top_mag;
   bad = __syncthreads_or(bad);
-  const int slot = threadIdx.x >> 1;
-  const unsigned long long* of = key;
-  int n = E;
-  if (E > kRankGroup) {  // at most eight groups, with k <= 16 candidates each
-    for (int g0 = 0; g0 < E; g0 += kRankGroup) {
-      const int gn = min(kRankGroup, E - g0);
-      const unsigned long long mine = key[g0 + min(slot, gn - 1)];
-      const int before = rank_of(key + g0, gn, mine);
-      if (slot < gn && !(threadIdx.x & 1) && before < k) cand[atomicAdd(&n_cand, 1)] = mine;
+#pragma unroll
+  for (int i = 0; i < kRouteWarps; ++i) top_mag = fmaxf(top_mag, warp_mag[i]);
+  const double tol = static_cast<double>(top_mag) * kLogitError;
+  for (bool exact = false;; exact = true) {
+    const int slot = threadIdx.x >> 1;
+    const unsigned long long* of = key;
+    int n = E;
+    if (E > kRankGroup) {  // at most eight groups, with k <= 16 candidates each
+      for (int g0 = 0; g0 < E; g0 += kRankGroup) {
+        const int gn = min(kRankGroup, E - g0);
+        const unsigned long long mine = key[g0 + min(slot, gn - 1)];
+        const int before = rank_of(key + g0, gn, mine);
+        if (slot < gn && !(threadIdx.x & 1) && before < k) cand[atomicAdd(&n_cand, 1)] = mine;
+      }
+      __syncthreads();
+      n = n_cand;
+      of = cand;
     }
+    const unsigned long long mine = of[min(slot, n - 1)];
+    const int before = rank_of(of, n, mine);
+    if (slot < n && !(threadIdx.x & 1) && before < k) chosen[before] = key_expert(mine);
     __syncthreads();
-    n = n_cand;
-    of = cand;
-  }
-  const unsigned long long mine = of[min(slot, n - 1)];
-  const int before = rank_of(of, n, mine);
-  if (slot < n && !(threadIdx.x & 1) && before < k) chosen[before] = key_expert(mine);
-  __syncthreads();
-  if (warp != 0) return;
-  const int my_e = lane < k ? chosen[lane] : chosen[0];
-  const double top = logits[chosen[0]];
-  const float p = expf(static_cast<float>(logits[my_e] - top));
-  float all = 0.f;
-  if (norm)
-    all = lane < k ? p : 0.f;
-  else
-    for (int e = lane; e < E; e += 32) all += expf(static_cast<float>(logits[e] - top));
-  all = warp_sum(all);
-  if (lane < k) {
-    w[static_cast<size_t>(t) * k + lane] = bad ? __int_as_float(0x7fffffff) : p / all;
-    idx[static_cast<size_t>(t) * k + lane] = my_e;
+    int close = 0;
+    if (warp == 0) {
+      const int my_e = lane < k ? chosen[lane] : chosen[0];
+      const double top = logits[chosen[0]];
+      const float p = expf(static_cast<float>(logits[my_e] - top));
+      float all = 0.f;
+      if (norm)
+        all = lane < k ? p : 0.f;
+      else
+        for (int e = lane; e < E; e += 32) all += expf(static_cast<float>(logits[e] - top));
+      all = warp_sum(all);
+      if (lane < k) {
+        w[static_cast<size_t>(t) * k + lane] = bad ? __int_as_float(0x7fffffff) : p / all;
+        idx[static_cast<size_t>(t) * k + lane] = my_e;
+      }
+    } else if (!exact) {  // whether the error of the sums could have made this order
+      const int i = threadIdx.x - 32;
+      const double last = logits[chosen[k - 1]];
+      const unsigned long long last_key = key[chosen[k - 1]];
+      close = i + 1 < k && logits[chosen[i]] - logits[chosen[i + 1]] <= tol;
+      for (int e = i; e < E; e += kRouteThreads - 32) close |= key[e] < last_key && logits[e] >= last - tol;
+    }
+    if (!__syncthreads_or(close)) return;
+    // the logits in question again in fp64, and once more: chosen ones beside a neighbour or the last one, others beside it
+    const double last = logits[chosen[k - 1]];
+    const unsigned long long last_key = key[chosen[k - 1]];
+    if (threadIdx.x == 0) n_cand = n_close = 0;
+    __syncthreads();
+    const int r = threadIdx.x;
+    if (r < k) {
+      const double z = logits[chosen[r]];
+      if (z - last <= tol || (r > 0 && logits[chosen[r - 1]] - z <= tol) || z - logits[chosen[min(r + 1, k - 1)]] <= tol)
+        near[atomicAdd(&n_close, 1)] = static_cast<unsigned short>(chosen[r]);
+    }
+    for (int e = threadIdx.x; e < E; e += kRouteThreads)
+      if (key[e] < last_key && logits[e] >= last - tol) near[atomicAdd(&n_close, 1)] = static_cast<unsigned short>(e);
+    __syncthreads();
+    const int n_near = n_close;
+    for (int c0 = 0; c0 < n_near; c0 += kExactBatch) {  // every thread takes eight columns of a batch of experts
+      double z[kExactBatch];
+      const __nv_bfloat16* row[kExactBatch];
+#pragma unroll
+      for (int j = 0; j < kExactBatch; ++j) {
+        z[j] = 0.0;
+        row[j] = rw + static_cast<size_t>(near[min(c0 + j, n_near - 1)]) * H;
+      }
+      for (int i = threadIdx.x * 8; i < H; i += 8 * kRouteThreads) {
+        const uint4 x8 = *reinterpret_cast<const uint4*>(h + static_cast<size_t>(t) * h_stride + i);
+        uint4 w8[kExactBatch];
+#pragma unroll
+        for (int j = 0; j < kExactBatch; ++j) w8[j] = __ldg(reinterpret_cast<const uint4*>(row[j] + i));
+#pragma unroll
+        for (int j = 0; j < kExactBatch; ++j) z[j] = dot8(x8, w8[j], z[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kExactBatch; ++j) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) z[j] += __shfl_xor_sync(0xffffffffu, z[j], o);
+        if (lane == 0) exact_part[j][warp] = z[j];
+      }
+      __syncthreads();
+      if (threadIdx.x < kExactBatch && c0 + static_cast<int>(threadIdx.x) < n_near) {
+        double v = 0.0;
+#pragma unroll
+        for (int i = 0; i < kRouteWarps; ++i) v += exact_part[threadIdx.x][i];
+        const int e = near[c0 + threadIdx.x];
+        logits[e] = v + 0.0;
+        key[e] = logit_key(v + 0.0, e);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -837,7 +936,7 @@ int sb_moe_few_route(const void* h, long long h_stride, const void* router, cons
     return SB_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(router)) & 15) return SB_ERR_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  sb::mf::route_kernel<<<(T + sb::mf::kCluster - 1) / sb::mf::kCluster * sb::mf::kCluster, sb::mf::kRouteThreads, sizeof(double) * E, st>>>(
+  sb::mf::route_kernel<<<(T + sb::mf::kCluster - 1) / sb::mf::kCluster * sb::mf::kCluster, sb::mf::kRouteThreads, (sizeof(double) + sizeof(float)) * E, st>>>(
       static_cast<const __nv_bfloat16*>(h), h_stride, static_cast<const __nv_bfloat16*>(router), live, w, idx, T, E, H, k, norm);
   return cudaGetLastError() == cudaSuccess ? SB_OK : SB_ERR_CUDA;
 }

@@ -87,6 +87,37 @@ def test_ties_nan_repeated_and_missing_experts():
     assert ((out.double() - want).abs() <= bound + 2.0**-8 * want.abs()).all() and not out[2].any()
 
 
+@pytest.mark.parametrize("E,H", [(40, 64), (128, 2048), (1000, 520)])
+def test_equal_logits_summed_in_other_orders(E, H):
+    """Experts whose weights are one another's in another order: all logits are equal, or one of two values, whatever
+    fp32 sums make of them."""
+    g = torch.Generator().manual_seed(E)
+    base = torch.randn(H, generator=g).to(BF)
+    rw = torch.stack([base[torch.randperm(H, generator=g)] for _ in range(E)]).cuda()
+    h = torch.tensor([1.0, -0.5, 2.0**-20], dtype=BF)[:, None].expand(3, H).contiguous().cuda()
+    w, idx = moe_few.route_few(h, rw, 8)
+    assert torch.equal(idx, torch.arange(8, device="cuda", dtype=torch.int32).expand(3, 8)) and (w - 0.125).abs().max() <= 2.0**-20
+    rw[1::2, 0] += torch.where(base.float().sum() < 0, -2.0, 2.0).to(BF).cuda()
+    for norm in (True, False):
+        w, idx = moe_few.route_few(h, rw, 3, norm)
+        w64, i64 = route64(h, rw, 3, norm)
+        assert torch.equal(idx.long(), i64) and (w.double() - w64).abs().max() <= 2.0**-20
+
+
+@pytest.mark.parametrize("E,H,k", [(40, 64, 8), (128, 2048, 3), (250, 4104, 16)])
+def test_logits_apart_by_less_than_a_sum_of_fp32_holds(E, H, k):
+    """Two large columns cancel; what is left orders the experts and lies below the last bit of the large ones."""
+    rw = torch.zeros(E, H, dtype=BF)
+    rw[:, 0], rw[:, 1] = 2.0**15, -(2.0**15)
+    rw[:, 2] = torch.tensor([e * 37 % E for e in range(E)]) * 2.0**-14
+    rw = rw.cuda()
+    for norm in (True, False):
+        h = torch.ones(9, H, device="cuda", dtype=BF)
+        w, idx = moe_few.route_few(h, rw, k, norm)
+        w64, i64 = route64(h, rw, k, norm)
+        assert torch.equal(idx.long(), i64) and (w.double() - w64).abs().max() <= 2.0**-20
+
+
 @pytest.mark.parametrize("E,H", [(40, 64), (300, 520)])
 def test_infinite_logits(E, H):
     """An expert with a logit of -inf is left out without spoiling its row; one of +inf comes first, and the weights are
