@@ -10,8 +10,8 @@
 // Bound by HBM: every row is read and written once (backward: gradient and input in, gradient out).  A lane owns whole
 // pairs of a head (16 elements, 8 in the pipeline for many rows), so that rotation needs no exchange and the norm only a
 // shuffle over a head's lanes; a warp holds several heads of one token at a time and loads the angles once for all.
-// Statistics, products and sums are fp32; rows are rounded once on store.  Three variants: plain loads for few rows, a
-// pipeline of bulk copies through shared memory for many, element by element for any size and alignment.
+// Statistics, products and sums are fp32; rows are rounded once on store.  Variants: plain loads for few rows (16 or 8
+// elements a lane), a pipeline of bulk copies through shared memory for many, element by element for any size and alignment.
 // Positions outside the table give NaN in the rotated elements instead of a read outside it.
 // 16384 rows of 32 + 4 + 4 heads of 128 in bf16: forward 60 us, 88% of the measured copy bandwidth; backward 90 us, 84%.
 #include <cuda_fp16.h>
@@ -188,7 +188,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
 // Few rows: a warp takes as many neighbouring heads of a token as fit its lanes, so that the call is one round of loads.
-template <typename T, bool kInter, bool kNorm, bool kPart>
+template <typename T, bool kInter, bool kNorm>
 __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -203,36 +203,9 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const Args a) {
   const bool on = u.live && h < a.heads, turned = h < a.nq + a.nk;
   Vec8<T> vlo, vhi;
   if (on) {
-    if (kPart) {
-      Sum lo[8], hi[8];
-      const float* p = static_cast<const float*>(a.src) + static_cast<size_t>(t) * a.src_stride + h * a.D;
-      for (int i = 0; i < a.n_part; ++i, p += a.part_stride) {
-        Vec8<float> l, r;
-        l.load(p + u.lo);
-        r.load(p + u.hi);
-        float fl[8], fr[8];
-        l.get(fl);
-        r.get(fr);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          lo[j].add(fl[j]);
-          hi[j].add(fr[j]);
-        }
-      }
-      float fl[8], fr[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        fl[j] = lo[j].get();
-        fr[j] = hi[j].get();
-      }
-      // the unsplit projection stores its rows in this type: keep that rounding, so that both paths agree
-      vlo.set(fl);
-      vhi.set(fr);
-    } else {
-      const T* p = static_cast<const T*>(a.src) + static_cast<size_t>(t) * a.src_stride + h * a.D;
-      vlo.load(p + u.lo);
-      vhi.load(p + u.hi);
-    }
+    const T* p = static_cast<const T*>(a.src) + static_cast<size_t>(t) * a.src_stride + h * a.D;
+    vlo.load(p + u.lo);
+    vhi.load(p + u.hi);
   }
   float cs[8], sn[8];
   if (u.rot) load_angles(a.table, a.pos[t], a.max_pos, a.R, c, cs, sn);
@@ -498,6 +471,19 @@ struct Spot {
   int lo, hi;    // first and second members of pairs 0 and 1; without kFine of all four
   int lo2, hi2;  // of pairs 2 and 3
 };
+template <bool kInter, bool kFine>
+__device__ __forceinline__ Spot spot_of(int c, int half, bool live, bool rot, bool rot2) {
+  Spot at;
+  at.lo = !live ? 0 : kInter || !rot ? 8 * c : 4 * c;
+  if (kFine) {
+    at.hi = rot ? half + 4 * c : at.lo + 2;
+    at.lo2 = !live ? 4 : rot2 ? 4 * c + 2 : 8 * c + 4;
+    at.hi2 = rot2 ? half + 4 * c + 2 : at.lo2 + 2;
+  } else {
+    at.hi = kInter || !rot ? at.lo + 4 : half + 4 * c;
+  }
+  return at;
+}
 template <typename T, bool kInter, bool kFine>
 __device__ __forceinline__ Pairs get_pairs(const T* p, const Spot& at) {
   Pairs v;
@@ -560,6 +546,117 @@ __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t 
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
 }
 
+// Angles of a rotating lane's four pairs at position p; 1 and 0 for pairs that do not rotate.
+template <bool kFine>
+__device__ __forceinline__ void load_angles4(const Args& a, int p, int c, bool rot2, float4& cs, float4& sn) {
+  if (p < 0 || p >= a.max_pos) {
+    const float nan = __int_as_float(0x7fffffff);
+    cs = rot2 ? make_float4(nan, nan, nan, nan) : make_float4(nan, nan, 1.f, 1.f);
+    sn = rot2 ? make_float4(nan, nan, nan, nan) : make_float4(nan, nan, 0.f, 0.f);
+    return;
+  }
+  const float* t = a.table + static_cast<size_t>(p) * a.R + 4 * c;
+  const float* u = t + (a.R >> 1);
+  if (kFine) {
+    const float2 c0 = __ldg(reinterpret_cast<const float2*>(t)), s0 = __ldg(reinterpret_cast<const float2*>(u));
+    float2 c1 = make_float2(1.f, 1.f), s1 = make_float2(0.f, 0.f);
+    if (rot2) {
+      c1 = __ldg(reinterpret_cast<const float2*>(t + 2));
+      s1 = __ldg(reinterpret_cast<const float2*>(u + 2));
+    }
+    cs = make_float4(c0.x, c0.y, c1.x, c1.y);
+    sn = make_float4(s0.x, s0.y, s1.x, s1.y);
+  } else {
+    cs = __ldg(reinterpret_cast<const float4*>(t));
+    sn = __ldg(reinterpret_cast<const float4*>(u));
+  }
+}
+
+// Few rows as in fwd_kernel, with eight elements a lane: for sizes that are no multiples of 16, for fp32 rows, where that
+// is 32 bytes, and for partial sums, where twice the lanes have the loads of twice the parts under way.
+template <typename T, bool kInter, bool kFine, bool kNorm, bool kPart>
+__global__ void __launch_bounds__(kThreads) fwd8_kernel(const Args a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long item = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (item >= static_cast<long long>(a.T) * a.blocks_per_row) return;
+  const int t = static_cast<int>(item / a.blocks_per_row);
+  const int blk = static_cast<int>(item - static_cast<long long>(t) * a.blocks_per_row);
+  const int c = lane & ((1 << a.log_group) - 1);
+  const int h = (blk << (5 - a.log_group)) + (lane >> a.log_group);
+  const int half = a.R >> 1;
+  const bool live = c * 8 < a.D, on = live && h < a.heads, turned = h < a.nq + a.nk;
+  const bool rot = c * 8 < a.R, rot2 = kFine ? 4 * c + 2 < half : rot;
+  const Spot at = spot_of<kInter, kFine>(c, half, live, rot, rot2);
+  Pairs v = {};
+  if (on) {
+    const size_t from = static_cast<size_t>(t) * a.src_stride + h * a.D;
+    if (kPart) {
+      Sum sum[8];
+      const float* p = static_cast<const float*>(a.src) + from;
+      for (int i = 0; i < a.n_part; ++i, p += a.part_stride) {
+        const Pairs q = get_pairs<float, kInter, kFine>(p, at);
+        float e[8];
+        unpack2(q.a[0], e[0], e[1]);
+        unpack2(q.a[1], e[2], e[3]);
+        unpack2(q.b[0], e[4], e[5]);
+        unpack2(q.b[1], e[6], e[7]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j].add(e[j]);
+      }
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = to_f(from_f<T>(sum[j].get()));
+      v.a[0] = pack2(e[0], e[1]);
+      v.a[1] = pack2(e[2], e[3]);
+      v.b[0] = pack2(e[4], e[5]);
+      v.b[1] = pack2(e[6], e[7]);
+    } else {
+      v = get_pairs<T, kInter, kFine>(static_cast<const T*>(a.src) + from, at);
+    }
+  }
+  float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (rot) load_angles4<kFine>(a, a.pos[t], c, rot2, cs, sn);
+  long long slot = a.slots ? a.slots[t] : -1;
+  if (slot >= a.n_slots) slot = -1;
+  if (kNorm) {
+    f2 s2 = mul2(v.a[0], v.a[0]);
+    s2 = fma2(v.b[0], v.b[0], s2);
+    s2 = fma2(v.a[1], v.a[1], s2);
+    s2 = fma2(v.b[1], v.b[1], s2);
+    const float ss = group_sum(on ? sum2(s2) : 0.f, a.log_group);
+    if (on && turned) {
+      const float r = rsqrtf(ss / static_cast<float>(a.D) + a.eps);
+      const f2 r2 = pack2(r, r);
+      const Pairs w = get_pairs<T, kInter, kFine>(static_cast<const T*>(h < a.nq ? a.qw : a.kw), at);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        v.a[j] = mul2(mul2(v.a[j], r2), w.a[j]);
+        v.b[j] = mul2(mul2(v.b[j], r2), w.b[j]);
+      }
+    }
+  }
+  if (!on) return;
+  if (turned && rot) {
+    const f2 cc[2] = {pack2(cs.x, cs.y), pack2(cs.z, cs.w)};
+    const f2 ss[2] = {pack2(sn.x * a.sign, sn.y * a.sign), pack2(sn.z * a.sign, sn.w * a.sign)};
+    const f2 ns[2] = {pack2(sn.x * -a.sign, sn.y * -a.sign), pack2(sn.z * -a.sign, sn.w * -a.sign)};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (j == 1 && !rot2) continue;  // not times 1 plus 0: there may be infinities
+      const f2 va = fma2(v.b[j], ns[j], mul2(v.a[j], cc[j]));
+      v.b[j] = fma2(v.a[j], ss[j], mul2(v.b[j], cc[j]));
+      v.a[j] = va;
+    }
+  }
+  if (h < a.store_heads)
+    put_pairs<T, kInter, kFine>(static_cast<T*>(a.dst) + static_cast<size_t>(t) * a.dst_stride + h * a.D, at, v);
+  if (slot >= 0 && h >= a.nq)
+    put_pairs<T, kInter, kFine>(
+        static_cast<T*>(turned ? a.kc : a.vc) + (static_cast<size_t>(slot) * a.nk + (turned ? h - a.nq : h - a.nq - a.nk)) * a.D, at, v);
+}
+
 constexpr int kStages = 3;
 constexpr int kRowWarps = 16;
 
@@ -587,15 +684,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
   const bool live = c * 8 < a.D, rot = c * 8 < a.R;  // a lane without elements goes along with the first one's
   const int half = a.R >> 1;
   const bool rot2 = kFine ? 4 * c + 2 < half : rot;  // pairs 2 and 3
-  Spot at;
-  at.lo = !live ? 0 : kInter || !rot ? 8 * c : 4 * c;
-  if (kFine) {
-    at.hi = rot && live ? half + 4 * c : at.lo + 2;
-    at.lo2 = !live ? 4 : rot2 ? 4 * c + 2 : 8 * c + 4;
-    at.hi2 = rot2 && live ? half + 4 * c + 2 : at.lo2 + 2;
-  } else {
-    at.hi = kInter || !rot ? at.lo + 4 : half + 4 * c;
-  }
+  const Spot at = spot_of<kInter, kFine>(c, half, live, rot, rot2);
   const int turned = a.nq + a.nk;
   const int head_bytes = a.D * static_cast<int>(sizeof(T));
   const int block_heads = piece_bytes / head_bytes;
@@ -639,26 +728,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
   float4 cos_next = make_float4(1.f, 1.f, 1.f, 1.f), sin_next = make_float4(0.f, 0.f, 0.f, 0.f);
   auto angles = [&](int p) {
     if (!rot) return;
-    if (p < 0 || p >= a.max_pos) {
-      const float nan = __int_as_float(0x7fffffff);
-      cos_next = rot2 ? make_float4(nan, nan, nan, nan) : make_float4(nan, nan, 1.f, 1.f);
-      sin_next = rot2 ? make_float4(nan, nan, nan, nan) : make_float4(nan, nan, 0.f, 0.f);
-      return;
-    }
-    const float* t = a.table + static_cast<size_t>(p) * a.R + 4 * c;
-    if (kFine) {
-      const float2 c0 = __ldg(reinterpret_cast<const float2*>(t)), s0 = __ldg(reinterpret_cast<const float2*>(t + half));
-      float2 c1 = make_float2(1.f, 1.f), s1 = make_float2(0.f, 0.f);
-      if (rot2) {
-        c1 = __ldg(reinterpret_cast<const float2*>(t + 2));
-        s1 = __ldg(reinterpret_cast<const float2*>(t + half + 2));
-      }
-      cos_next = make_float4(c0.x, c0.y, c1.x, c1.y);
-      sin_next = make_float4(s0.x, s0.y, s1.x, s1.y);
-    } else {
-      cos_next = __ldg(reinterpret_cast<const float4*>(t));
-      sin_next = __ldg(reinterpret_cast<const float4*>(t + half));
-    }
+    load_angles4<kFine>(a, p, c, rot2, cos_next, sin_next);
   };
   if (count > 0) angles(p_first);
 
@@ -1059,32 +1129,41 @@ cudaError_t launch_rows(const Args& a, int ctas, cudaStream_t st) {
 // From how many bytes of rows on the pipeline is taken.  Below, its start (4 us against 2) costs more than it gains, and
 // rows that lie in L2 come fast enough through plain loads.  bf16, 40 heads of 128, plain kernel / pipeline in us: forward
 // of 23 MB 12.1 / 13.5, of 47 MB 28.3 / 23.5, of 160 MB 89.7 / 60.0; backward of 0.6 MB 6.2 / 6.8, of 1.5 MB 8.7 / 7.0, of
-// 160 MB 144 / 90.  Head sizes and widths that would go element by element otherwise, where the number of elements counts:
-// 8 + 2 + 2 heads of 80, 40 rotated, element by element / pipeline: forward of 0.5 M elements 4.1 / 4.8, of 1 M 6.3 / 4.9,
-// of 16 M 79 / 20; backward of 0.25 M 7.8 / 8.5, of 0.5 M 10.3 / 8.7, of 16 M 146 / 30.
+// 160 MB 144 / 90.  Head sizes and widths that are no multiples of 16: 8 + 2 + 2 heads of 80, 40 rotated, plain / pipeline,
+// forward of 1 M elements 3.4 / 4.8, of 2 M 5.4 / 4.9, of 16 M 33 / 20, in fp32 of 2 M 5.2 / 5.9, of 4 M 9.0 / 8.9; backward,
+// element by element / pipeline, of 0.25 M 7.8 / 8.5, of 0.5 M 10.3 / 8.7, of 16 M 146 / 30.
 constexpr long long kForwardFrom = 28LL << 20, kBackwardFrom = 640LL << 10;
-constexpr long long kForwardFromElements = 800LL << 10, kBackwardFromElements = 350LL << 10;
+constexpr long long kForwardFromElements = 1LL << 20, kBackwardFromElements = 175LL << 10;  // per byte of an element
 bool row_pipeline(const Args& a, size_t elt, long long from, long long from_elements) {
   if (a.D > 256 || !vectorised(a, elt, 8, 4)) return false;
-  const long long elements = static_cast<long long>(a.T) * a.heads * a.D;
-  return vectorised(a, elt, 16, 16) ? elements * static_cast<long long>(elt) > from : elements > from_elements;
+  const long long e = static_cast<long long>(elt), elements = static_cast<long long>(a.T) * a.heads * a.D;
+  return vectorised(a, elt, 16, 16) ? elements * e > from : elements > from_elements * e;
 }
 
 template <typename T, bool kInter, bool kNorm, bool kPart>
 cudaError_t launch_fwd(Args a, cudaStream_t st) {
   if (!kPart && row_pipeline(a, sizeof(T), kForwardFrom, kForwardFromElements))
     return launch_rows<T, kInter, kNorm ? kNormRotate : kRotate>(a, sm_count(), st);
-  if (!vectorised(a, sizeof(T), 16, 16)) {
+  // 16 elements a lane where that is the faster form (us, 16 / 8 elements a lane, 32 + 4 + 4 heads of 128): bf16 rows, 64
+  // 2.5 / 2.4, 1024 6.4 / 8.1, 2048 10.5 / 14.3; fp32 rows of 8 + 4 + 4 heads of 256, 256 4.4 / 3.6, 2048 13.9 / 13.3; four
+  // partial sums, 64 rows 4.4 / 3.7, 512 rows 11.7 / 9.3.
+  const bool wide = !kPart && vectorised(a, sizeof(T), 16, 16) && (sizeof(T) == 2 || a.D > 256);
+  if (!wide && (a.D > 256 || !vectorised(a, sizeof(T), 8, 4))) {
     const long long ctas = (static_cast<long long>(a.T) * a.heads + kWarps - 1) / kWarps;
     if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_pdl(fwd_any_kernel<T, kInter, kNorm, kPart>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0, st, a);
   }
-  a.log_group = log2_ceil(a.D / 16);
+  a.log_group = log2_ceil(wide ? a.D / 16 : a.D / 8);
   const int hpw = 32 >> a.log_group;
   a.blocks_per_row = (a.heads + hpw - 1) / hpw;  // every pass over heads on a warp of its own: the call is one round of loads
   const long long ctas = (static_cast<long long>(a.T) * a.blocks_per_row + kWarps - 1) / kWarps;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-  return launch_pdl(fwd_kernel<T, kInter, kNorm, kPart>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0, st, a);
+  const dim3 grid(static_cast<unsigned>(ctas));
+  if constexpr (!kPart) {
+    if (wide) return launch_pdl(fwd_kernel<T, kInter, kNorm>, grid, dim3(kThreads), 0, st, a);
+  }
+  if (a.R % 8) return launch_pdl(fwd8_kernel<T, kInter, true, kNorm, kPart>, grid, dim3(kThreads), 0, st, a);
+  return launch_pdl(fwd8_kernel<T, kInter, false, kNorm, kPart>, grid, dim3(kThreads), 0, st, a);
 }
 
 template <typename T>
