@@ -421,13 +421,17 @@ __device__ __forceinline__ Unit unit_at(const Lists& L, int unit) {
 // memory.  A ring of stages takes a block each (or a piece of at most kMaxPiece columns of it); one lane fills it with
 // bulk copies as far ahead as the ring is long, a whole block in a copy where it fits: a copy costs the engine about 90
 // cycles whatever its size: rows of 1.5 KB one by one came at 4.8 TB/s, blocks of 16 to 32 KB come at 6.7 to 6.9.
-// Eight warps take a share of every piece's columns each; their sums meet in shared memory at the end of the item.
+// The consumers are groups of kGroup warps; each group takes the next item on, its warps a share of the columns each, and
+// their sums meet in shared memory at the end of the item.  A warp's share is at most eight k steps, so that wide rows
+// need all eight warps; narrow ones leave groups that hide one another's barriers (64 tokens, 128 experts of 1024 x 512,
+// top 8, gate and up: 66 us with one group, 52 with two).
 // ---------------------------------------------------------------------------
 constexpr int kConsumers = 8;
 constexpr int kConsumerThreads = 32 * kConsumers;
 constexpr int kRingThreads = kConsumerThreads + 32;
 constexpr int kMaxStages = 24;
-constexpr int kMaxPiece = 2048;  // columns; a warp's share is at most 8 k steps of 32
+constexpr int kSteps = 8;         // k steps of 32 columns, at most, of a warp's share
+constexpr int kMaxPiece = 32 * kSteps * kConsumers;  // columns
 constexpr int kMaxNt = kUnitRows / 8;
 constexpr int kRedBytes = 2 * kConsumers * kMaxNt * 32 * 16;  // sums of two items
 
@@ -458,7 +462,13 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 // Weights that other kernels wrote through ordinary stores are read by bulk copies.
 __device__ __forceinline__ void fence_proxy_async_global() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
-__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumerThreads) : "memory"); }
+template <int kGroup>
+__device__ __forceinline__ void group_sync(int group) {
+  if (kGroup == 1)
+    __syncwarp();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * kGroup) : "memory");
+}
 
 // Fill the stages of one item (called by a whole warp): blocks of rows_a rows at a and rows_b rows at b.  Returns false
 // when a wait gave up.
@@ -483,21 +493,22 @@ __device__ __forceinline__ bool produce_item(Ring& ring, char* buf, const Shape&
   return true;
 }
 
-// The consumers' loop over `items` items.  unit_of() gives the unit of the next item, row_ptr(r) the operand row of entry
-// r, finish(unit, sums) takes the warps' sums [warp][column group][lane] of an item.  A warp's share of the operand rows
+// A group's loop over its items, every (kConsumers / kGroup)-th of `items`.  unit_of() gives the unit of its next item,
+// row_ptr(r) the operand row of entry r, finish(unit, sums) takes the warps' sums [warp][column group][lane] of an item.  A warp's share of the operand rows
 // stays in registers from item to item of a unit (rows of more than one piece: from L1 or L2 again).
-template <int kNt, int kSteps, class UnitOf, class RowPtr, class Finish>
+template <int kNt, int kGroup, class UnitOf, class RowPtr, class Finish>
 __device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red, const Shape& s, int items, int* status,
                                         UnitOf unit_of, RowPtr row_ptr, Finish finish) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kGroups = kConsumers / kGroup;
+  const int lane = threadIdx.x & 31, group = threadIdx.x / (32 * kGroup), warp = (threadIdx.x >> 5) % kGroup;
   const int g = lane >> 2, t4 = lane & 3;
   // k steps of piece q that fall to this warp: `mine` from `lo`; the first `some` of them have columns for this lane
   int lo = 0, mine = 0, some = 0;
   auto share = [&](int q) {
     const int cols = min(s.piece, s.K - q * s.piece);
     const int steps = (cols + 31) >> 5;
-    lo = warp * steps / kConsumers;
-    mine = (warp + 1) * steps / kConsumers - lo;
+    lo = warp * steps / kGroup;
+    mine = (warp + 1) * steps / kGroup - lo;
     some = min(mine, max(0, (cols - lo * 32 - 8 * t4 + 31) >> 5));
   };
   share(0);
@@ -512,9 +523,11 @@ __device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red
         v[j][n] = j < some && x[n] ? *reinterpret_cast<const uint4*>(x[n] + at + j * 32) : make_uint4(0, 0, 0, 0);
   };
   Turn turn;
+  for (int i = 0; i < 2 * group; ++i) turn.step(s.stages);  // more than one group: rows of one piece
   int r0 = -1;
   bool ok = true;  // after a wait gave up, the items are run through without waiting: every warp still meets the others
-  for (int i = 0; i < items; ++i) {
+  float4* sums = red + group * (2 * kGroup * kNt * 32);
+  for (int i = group; i < items; i += kGroups) {
     const Unit u = unit_of();
     float acc[kNt][4];
 #pragma unroll
@@ -562,29 +575,31 @@ __device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red
         mbar_arrive(free_b);
       }
     }
+#pragma unroll
+    for (int skip = 0; skip < 2 * (kGroups - 1); ++skip) turn.step(s.stages);
     // two buffers: an item's sums are read while the next item's are not yet all written, so one barrier an item is enough
-    float4* sums = red + (i & 1) * (kConsumers * kNt * 32);
 #pragma unroll
     for (int n = 0; n < kNt; ++n) sums[(warp * kNt + n) * 32 + lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-    consumer_sync();
+    group_sync<kGroup>(group);
     finish(u, sums);
+    sums = red + group * (2 * kGroup * kNt * 32) + (sums == red + group * (2 * kGroup * kNt * 32) ? kGroup * kNt * 32 : 0);
   }
 }
 
 // Sum over the warps of component c of column group n's fragment in lane l.
-template <int kNt>
+template <int kNt, int kGroup>
 __device__ __forceinline__ float warp_total(const float4* sums, int n, int l, int c) {
   float v = 0.f;
 #pragma unroll
-  for (int w = 0; w < kConsumers; ++w) v += reinterpret_cast<const float*>(&sums[(w * kNt + n) * 32 + l])[c];
+  for (int w = 0; w < kGroup; ++w) v += reinterpret_cast<const float*>(&sums[(w * kNt + n) * 32 + l])[c];
   return v;
 }
 
-__device__ __forceinline__ void ring_init(Ring& ring, int stages) {
+__device__ __forceinline__ void ring_init(Ring& ring, int stages, int group_warps) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; ++i) {
       mbar_init(&ring.full[i], 1);
-      mbar_init(&ring.empty[i], kConsumers);
+      mbar_init(&ring.empty[i], group_warps);
     }
     fence_mbar_init();
   }
@@ -602,7 +617,7 @@ __device__ __forceinline__ void ring_drain(Ring& ring, const Shape& s, Turn turn
 // Gate and up projections: an item is eight gate rows and the eight up rows beside them, so that a lane holds both
 // factors of an activation.
 // ---------------------------------------------------------------------------
-template <int kSteps>
+template <int kGroup>
 __global__ void __launch_bounds__(kRingThreads, 1)
 gate_up_kernel(const __nv_bfloat16* h, long long h_stride, const int* idx, const __nv_bfloat16* __restrict__ wgu,
                __nv_bfloat16* act, int n, int k, int E, int H, int F, Shape s, int* status) {
@@ -610,7 +625,7 @@ gate_up_kernel(const __nv_bfloat16* h, long long h_stride, const int* idx, const
   extern __shared__ __align__(128) char smem[];
   float4* red = reinterpret_cast<float4*>(smem);
   char* buf = smem + kRedBytes;
-  ring_init(ring, s.stages);
+  ring_init(ring, s.stages, kGroup);
   pdl_wait();
   pdl_launch_dependents();
   const Lists L = build_lists(buf + static_cast<size_t>(s.stages) * 16 * s.piece, idx, n, E);
@@ -636,29 +651,36 @@ gate_up_kernel(const __nv_bfloat16* h, long long h_stride, const int* idx, const
   }
   auto run = [&](auto nt) {
     constexpr int kNt = decltype(nt)::value;
-    int unit = lo / tiles, tile = lo - unit * tiles - 1, f0 = 0;
+    constexpr int kGroups = kConsumers / kGroup;
+    const int group = threadIdx.x / (32 * kGroup), first = lo + group;
+    int unit = first / tiles, tile = first - unit * tiles - kGroups, f0 = 0;
     Unit u = {};
-    if (lo < hi) u = unit_at(L, unit);
+    if (first < hi) u = unit_at(L, unit);
     auto unit_of = [&]() {
-      if (++tile == tiles) {
-        tile = 0;
-        u = unit_at(L, ++unit);
+      tile += kGroups;
+      if (tile >= tiles) {
+        do {
+          tile -= tiles;
+          ++unit;
+        } while (tile >= tiles);
+        u = unit_at(L, unit);
       }
       f0 = tile * 8;
       return u;
     };
     auto row_ptr = [&](int r) { return h + static_cast<size_t>(L.entry[r] / k) * h_stride; };
     auto finish = [&](const Unit& v, const float4* sums) {
-      const int o = threadIdx.x;  // (column group, lane of the fragment, one of its two columns)
-      if (o >= kNt * 64) return;
-      const int c = o & 1, l = (o >> 1) & 31, grp = o >> 6;
-      const int r = v.r0 + grp * 8 + 2 * (l & 3) + c, f = f0 + (l >> 2);
-      if (r >= v.r1 || f >= F) return;
-      const float gate = warp_total<kNt>(sums, grp, l, c), up = warp_total<kNt>(sums, grp, l, 2 + c);
-      // the activation is the down product's bf16 operand, rounded here as on the path for many tokens
-      act[static_cast<size_t>(L.entry[r]) * F + f] = __float2bfloat16_rn(gate / (1.f + __expf(-gate)) * up);
+      // (column group, lane of the fragment, one of its two columns)
+      for (int o = threadIdx.x % (32 * kGroup); o < kNt * 64; o += 32 * kGroup) {
+        const int c = o & 1, l = (o >> 1) & 31, grp = o >> 6;
+        const int r = v.r0 + grp * 8 + 2 * (l & 3) + c, f = f0 + (l >> 2);
+        if (r >= v.r1 || f >= F) continue;
+        const float gate = warp_total<kNt, kGroup>(sums, grp, l, c), up = warp_total<kNt, kGroup>(sums, grp, l, 2 + c);
+        // the activation is the down product's bf16 operand, rounded here as on the path for many tokens
+        act[static_cast<size_t>(L.entry[r]) * F + f] = __float2bfloat16_rn(gate / (1.f + __expf(-gate)) * up);
+      }
     };
-    consume<kNt, kSteps>(ring, buf, red, s, hi - lo, status, unit_of, row_ptr, finish);
+    consume<kNt, kGroup>(ring, buf, red, s, hi - lo, status, unit_of, row_ptr, finish);
   };
   if (L.most <= 8)
     run(std::integral_constant<int, 1>());
@@ -667,7 +689,9 @@ gate_up_kernel(const __nv_bfloat16* h, long long h_stride, const int* idx, const
 }
 
 // ---------------------------------------------------------------------------
-// Down projection and combination.  A CTA owns 16 columns of the output for all tokens.  Its warps take the units in turn,
+// Down projection and combination.  A CTA owns 16 columns of the output for all tokens; where there are fewer such columns
+// than SMs, the CTAs of a cluster share them, each with a part of the units and, at the end, of the tokens (34 tokens, 104
+// experts of 552 x 560, top 7: 33 us with a CTA for 16 columns, 18 with three).  Its warps take the units in turn,
 // one each, with the weights straight from global memory into fragments: 16 warps with 16 loads a lane keep 128 KB a SM
 // under way, and no warp waits for another.  The entries' results stay in shared memory until all are there and are then
 // added up slot by slot, so no sum crosses a CTA.
@@ -683,7 +707,7 @@ __device__ __forceinline__ uint4 ld_stream(const __nv_bfloat16* p) {
 
 template <int kNt>
 __device__ __forceinline__ void down_unit(const Lists& L, float* y, const __nv_bfloat16* act, const __nv_bfloat16* wd, const Unit& u,
-                                          int n0, int H, int F) {
+                                          int n0, int H, int F, int k, int size) {
   const int lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   constexpr int kUnroll = kNt == 1 ? 8 : 4;
@@ -727,18 +751,22 @@ __device__ __forceinline__ void down_unit(const Lists& L, float* y, const __nv_b
     for (int col = 0; col < 2; ++col) {
       const int r = u.r0 + n * 8 + 2 * t4 + col;
       if (r < u.r1) {
-        float* o = y + L.entry[r] * 16;
+        const int entry = L.entry[r];
+        float* o = y + entry * 16;
+        if (size > 1) o = cg::this_cluster().map_shared_rank(o, entry / k % size);  // the CTA that combines this token
         o[g] = acc[n][col];
         o[g + 8] = acc[n][2 + col];
       }
     }
 }
 
-// The combination of a CTA's 16 columns from y [T * k][16]: slot by slot, so that the order is always the same.
+// The combination of a CTA's 16 columns from y [T * k][16], for every `of`-th token from `first` on: slot by slot, so that
+// the order is always the same.
 __device__ __forceinline__ void combine(const float* y, const int* idx, const float* w, __nv_bfloat16* out, int n0, int T, int k,
-                                        int E, int H) {
-  for (int i = threadIdx.x; i < T * 16; i += kDownThreads) {
-    const int t = i >> 4, c = i & 15;
+                                        int E, int H, int first, int of) {
+  for (int i = threadIdx.x;; i += kDownThreads) {
+    const int t = (i >> 4) * of + first, c = i & 15;
+    if (t >= T) break;
     if (n0 + c >= H) continue;
     float v = 0.f;
     for (int j = 0; j < k; ++j) {
@@ -753,19 +781,26 @@ __global__ void __launch_bounds__(kDownThreads, 1)
 down_kernel(const __nv_bfloat16* act, const int* __restrict__ idx, const float* w, const __nv_bfloat16* __restrict__ wd,
             __nv_bfloat16* __restrict__ out, int T, int k, int E, int H, int F) {
   extern __shared__ __align__(128) char smem[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int size = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  if (size > 1) cluster.barrier_arrive();
   const int n = T * k;
-  float* y = reinterpret_cast<float*>(smem);  // [n][16]
+  float* y = reinterpret_cast<float*>(smem);  // [n][16]; of the tokens that fall to this CTA
   const Lists L = build_lists(smem + sizeof(float) * 16 * static_cast<size_t>(n), idx, n, E);
-  const int n0 = blockIdx.x * 16;
-  for (int i = threadIdx.x >> 5; i < L.n_units; i += kDownThreads / 32) {
+  const int n0 = static_cast<int>(blockIdx.x) / size * 16;
+  if (size > 1) cluster.barrier_wait();  // every CTA of the cluster runs before its shared memory is written
+  for (int i = (threadIdx.x >> 5) * size + rank; i < L.n_units; i += kDownThreads / 32 * size) {
     const Unit u = unit_at(L, i);
     if (u.r1 - u.r0 <= 8)
-      down_unit<1>(L, y, act, wd, u, n0, H, F);
+      down_unit<1>(L, y, act, wd, u, n0, H, F, k, size);
     else
-      down_unit<2>(L, y, act, wd, u, n0, H, F);
+      down_unit<2>(L, y, act, wd, u, n0, H, F, k, size);
   }
-  __syncthreads();
-  combine(y, idx, w, out, n0, T, k, E, H);
+  if (size > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  combine(y, idx, w, out, n0, T, k, E, H, rank, size);
 }
 
 // The same for so few entries that all weights a CTA needs fit into its shared memory at once (one token with eight experts
@@ -868,7 +903,7 @@ down_once_kernel(const __nv_bfloat16* act, const int* idx, const float* w, const
       once_unit<2>(L, y, mine, rows, u, n_rows, F);
   }
   __syncthreads();
-  combine(y, idx, w, out, n0, T, k, E, H);
+  combine(y, idx, w, out, n0, T, k, E, H, 0, 1);
 }
 
 // Stages of eight rows of K columns in `room` bytes.  A row of more than kMaxPiece columns comes in equal pieces.
@@ -882,17 +917,17 @@ inline Shape ring_shape(int K, size_t room) {
   return s;
 }
 
-template <int kSteps>
+template <int kGroup>
 cudaError_t launch_gate_up(const void* h, long long h_stride, const int* idx, const void* wgu, void* act, int T, int k, int E, int H,
                            int F, const Shape& s, size_t smem, size_t smem_most, int* status, cudaStream_t st) {
   static bool attr_dev[64] = {};
   bool& attr = attr_dev[device_index()];
   if (!attr) {
-    const cudaError_t e = cudaFuncSetAttribute(gate_up_kernel<kSteps>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_most));
+    const cudaError_t e = cudaFuncSetAttribute(gate_up_kernel<kGroup>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_most));
     if (e != cudaSuccess) return e;
     attr = true;
   }
-  return launch_pdl(gate_up_kernel<kSteps>, dim3(sm_count()), dim3(kRingThreads), smem, st, static_cast<const __nv_bfloat16*>(h), h_stride,
+  return launch_pdl(gate_up_kernel<kGroup>, dim3(sm_count()), dim3(kRingThreads), smem, st, static_cast<const __nv_bfloat16*>(h), h_stride,
                     idx, static_cast<const __nv_bfloat16*>(wgu), static_cast<__nv_bfloat16*>(act), T * k, k, E, H, F, s, status);
 }
 
@@ -905,10 +940,33 @@ cudaError_t launch_down(const void* act, const int* idx, const float* w, const v
     if (e != cudaSuccess) return e;
     attr = true;
   }
-  down_kernel<<<(H + 15) / 16, kDownThreads, smem, st>>>(static_cast<const __nv_bfloat16*>(act), idx, w,
-                                                         static_cast<const __nv_bfloat16*>(wd), static_cast<__nv_bfloat16*>(out), T, k,
-                                                         E, H, F);
-  return cudaGetLastError();
+  constexpr int kMaxCluster = 8;
+  static int most_dev[64][kMaxCluster] = {};
+  int* clusters = most_dev[device_index()];  // of 1 to 8 CTAs that run at once
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kDownThreads);
+  cfg.dynamicSmemBytes = smem_most;
+  cudaLaunchAttribute shape[1];
+  shape[0].id = cudaLaunchAttributeClusterDimension;
+  cfg.attrs = shape;
+  cfg.numAttrs = 1;
+  for (unsigned i = 1; i <= kMaxCluster && clusters[kMaxCluster - 1] == 0; ++i) {
+    shape[0].val.clusterDim = {i, 1, 1};
+    cfg.gridDim = dim3(i);
+    int fit = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&fit, down_kernel, &cfg);
+    if (e != cudaSuccess) return e;
+    clusters[i - 1] = fit > 0 ? fit : 1;
+  }
+  const int tiles = (H + 15) / 16;
+  unsigned size = 1;  // as many CTAs as run in one wave
+  while (size < kMaxCluster && tiles <= clusters[size]) ++size;
+  shape[0].val.clusterDim = {size, 1, 1};
+  cfg.gridDim = dim3(tiles * size);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  return cudaLaunchKernelEx(&cfg, down_kernel, static_cast<const __nv_bfloat16*>(act), idx, w, static_cast<const __nv_bfloat16*>(wd),
+                            static_cast<__nv_bfloat16*>(out), T, k, E, H, F);
 }
 
 cudaError_t launch_down_once(const void* act, const int* idx, const float* w, const void* wd, void* out, int T, int k, int E, int H,
@@ -961,9 +1019,13 @@ int sb_moe_few_experts(const void* h, long long h_stride, const float* w, const 
   const sb::mf::Shape gu = sb::mf::ring_shape(H, most - fixed);
   if (gu.stages < 2) return SB_ERR_TOO_LARGE;
   const size_t smem_gu = fixed + static_cast<size_t>(gu.stages) * 16 * gu.piece;
-  // a warp's k steps of a piece: registers for four hold up to 1024 columns
-  cudaError_t e = (gu.piece <= 1024 ? sb::mf::launch_gate_up<4> : sb::mf::launch_gate_up<8>)(h, h_stride, idx, wgu, act, T, k, E, H, F, gu,
-                                                                                              smem_gu, most, status, st);
+  // as few warps a group as the columns allow
+  const int steps = (gu.piece + 31) / 32, per = sb::mf::kSteps;
+  const auto launch = gu.pieces > 1 || steps > 4 * per ? sb::mf::launch_gate_up<8>
+                      : steps > 2 * per                ? sb::mf::launch_gate_up<4>
+                      : steps > per                    ? sb::mf::launch_gate_up<2>
+                                                       : sb::mf::launch_gate_up<1>;
+  cudaError_t e = launch(h, h_stride, idx, wgu, act, T, k, E, H, F, gu, smem_gu, most, status, st);
   if (e != cudaSuccess) return SB_ERR_CUDA;
   const size_t once = sb::mf::once_bytes(n, F) + lists;
   if (n <= sb::mf::kOnceUnits && once <= most)

@@ -32,6 +32,7 @@ SIZES = [  # T, E, k, H, F
     (33, 8, 2, 256, 128), (64, 128, 8, 256, 64), (5, 1, 1, 8, 8), (3, 1024, 16, 64, 16), (100, 20, 5, 72, 40), (256, 16, 8, 64, 32),
     (19, 200, 1, 1024, 768), (5, 8, 2, 4104, 1032), (20, 6, 3, 2056, 40), (40, 3, 2, 6152, 24), (3, 4, 2, 2048, 2048),
     (20, 1, 1, 72, 40), (32, 2, 1, 136, 24), (33, 2, 1, 136, 24), (1, 128, 8, 2048, 768), (4, 16, 8, 264, 176),
+    (34, 30, 7, 552, 136), (19, 12, 3, 1000, 72), (30, 9, 4, 104, 520), (25, 40, 2, 1016, 264), (50, 4, 2, 8, 1032), (37, 7, 5, 496, 200),
 ]
 
 
