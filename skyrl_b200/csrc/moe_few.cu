@@ -422,16 +422,17 @@ __device__ __forceinline__ Unit unit_at(const Lists& L, int unit) {
 // bulk copies as far ahead as the ring is long, a whole block in a copy where it fits: a copy costs the engine about 90
 // cycles whatever its size: rows of 1.5 KB one by one came at 4.8 TB/s, blocks of 16 to 32 KB come at 6.7 to 6.9.
 // The consumers are groups of kGroup warps; each group takes the next item on, its warps a share of the columns each, and
-// their sums meet in shared memory at the end of the item.  A warp's share is at most eight k steps, so that wide rows
-// need all eight warps; narrow ones leave groups that hide one another's barriers (64 tokens, 128 experts of 1024 x 512,
-// top 8, gate and up: 66 us with one group, 52 with two).
+// their sums meet in shared memory at the end of the item.  A warp's share stays in registers, so that wide rows need all
+// eight warps; narrow ones leave groups that hide one another's barriers (gate and up of 64 tokens, 128 experts of
+// 1024 x 512, top 8: 66 us with one group, 51 with two; of 28 tokens, 159 experts of 1288 x 728: 89 and 81).
 // ---------------------------------------------------------------------------
 constexpr int kConsumers = 8;
 constexpr int kConsumerThreads = 32 * kConsumers;
 constexpr int kRingThreads = kConsumerThreads + 32;
 constexpr int kMaxStages = 24;
-constexpr int kSteps = 8;         // k steps of 32 columns, at most, of a warp's share
-constexpr int kMaxPiece = 32 * kSteps * kConsumers;  // columns
+constexpr int kMaxPiece = 2048;  // columns
+// k steps of 32 columns, at most, of a warp's share: more than twelve spill with 16 rows a unit
+__host__ __device__ constexpr int max_steps(int group) { return group == kConsumers ? kMaxPiece / 32 / kConsumers : 12; }
 constexpr int kMaxNt = kUnitRows / 8;
 constexpr int kRedBytes = 2 * kConsumers * kMaxNt * 32 * 16;  // sums of two items
 
@@ -499,7 +500,7 @@ __device__ __forceinline__ bool produce_item(Ring& ring, char* buf, const Shape&
 template <int kNt, int kGroup, class UnitOf, class RowPtr, class Finish>
 __device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red, const Shape& s, int items, int* status,
                                         UnitOf unit_of, RowPtr row_ptr, Finish finish) {
-  constexpr int kGroups = kConsumers / kGroup;
+  constexpr int kGroups = kConsumers / kGroup, kSteps = max_steps(kGroup);
   const int lane = threadIdx.x & 31, group = threadIdx.x / (32 * kGroup), warp = (threadIdx.x >> 5) % kGroup;
   const int g = lane >> 2, t4 = lane & 3;
   // k steps of piece q that fall to this warp: `mine` from `lo`; the first `some` of them have columns for this lane
@@ -1020,11 +1021,11 @@ int sb_moe_few_experts(const void* h, long long h_stride, const float* w, const 
   if (gu.stages < 2) return SB_ERR_TOO_LARGE;
   const size_t smem_gu = fixed + static_cast<size_t>(gu.stages) * 16 * gu.piece;
   // as few warps a group as the columns allow
-  const int steps = (gu.piece + 31) / 32, per = sb::mf::kSteps;
-  const auto launch = gu.pieces > 1 || steps > 4 * per ? sb::mf::launch_gate_up<8>
-                      : steps > 2 * per                ? sb::mf::launch_gate_up<4>
-                      : steps > per                    ? sb::mf::launch_gate_up<2>
-                                                       : sb::mf::launch_gate_up<1>;
+  const int steps = (gu.piece + 31) / 32;
+  const auto launch = gu.pieces > 1 || steps > 4 * sb::mf::max_steps(4) ? sb::mf::launch_gate_up<8>
+                      : steps > 2 * sb::mf::max_steps(2)                ? sb::mf::launch_gate_up<4>
+                      : steps > sb::mf::max_steps(1)                    ? sb::mf::launch_gate_up<2>
+                                                                        : sb::mf::launch_gate_up<1>;
   cudaError_t e = launch(h, h_stride, idx, wgu, act, T, k, E, H, F, gu, smem_gu, most, status, st);
   if (e != cudaSuccess) return SB_ERR_CUDA;
   const size_t once = sb::mf::once_bytes(n, F) + lists;
