@@ -93,7 +93,8 @@ def moe_ffn(h: torch.Tensor, router_w: torch.Tensor, wgu: torch.Tensor, wd: torc
     rows whose result is not used where it is 0; on the path for few tokens they read no expert and come out zero."""
     T, H = h.shape
     E = wgu.shape[0]
-    few = _takes_few(h, router_w, wgu, wd, top_k)
+    quantised = qat is not None and qat.enabled and torch.is_grad_enabled()
+    few = not quantised and _takes_few(h, router_w, wgu, wd, top_k)
     if few:
         w, idx = moe_few.route_few(h, router_w, top_k, norm_topk_prob, live=live)
     else:
@@ -114,7 +115,7 @@ def moe_ffn(h: torch.Tensor, router_w: torch.Tensor, wgu: torch.Tensor, wd: torc
     # rows grouped by expert, every expert's range padded to whole 128-row tiles (padding rows are zero)
     x = gg.dispatch_rows(h, plan)
     w1, w2 = wgu, wd
-    if qat is not None and qat.enabled and torch.is_grad_enabled():  # fake-INT4 expert weights, straight-through
+    if quantised:  # fake-INT4 expert weights, straight-through
         from .qat import fake_int4
 
         w1 = fake_int4(w1, qat.group_size, True, qat.scale_divisor, qat.q_min)

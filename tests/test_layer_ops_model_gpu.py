@@ -1,6 +1,7 @@
 """Rotary variants, head norms, cache rows, paged layout and few-token experts together in models and engine on the GPU."""
 import contextlib
 import dataclasses
+import types
 
 import pytest
 import torch
@@ -158,3 +159,15 @@ def test_replayed_routing_with_gaps_and_dead_rows():
     assert not out[1].any() and torch.equal(out[[0, 3, 4, 5]], forced[[0, 3, 4, 5]])
     # the row's own weights are taken from the replay's softmax (2^-20 of a weight apart, then one bf16 rounding)
     assert ((out[2] - own[2]).abs() <= 2.0**-7 * own[2].abs().max()).all() and torch.isfinite(out).all()
+
+
+def test_fake_int4_experts_are_not_taken_by_the_path_for_few_tokens():
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    h, rw, wgu, wd = r(6, 128), r(8, 128), r(8, 128, 128) / 11, r(8, 128, 64) / 8
+    qat = types.SimpleNamespace(enabled=True, group_size=32, scale_divisor=7.0, q_min=-7.0)
+    frozen = moe.moe_ffn(h, rw, wgu, wd, 2, qat=qat)  # gradients are on, nothing needs one
+    trained = moe.moe_ffn(h, rw, wgu.requires_grad_(), wd.requires_grad_(), 2, qat=qat)
+    assert torch.equal(frozen, trained)
+    with torch.no_grad():
+        assert not torch.equal(frozen, moe.moe_ffn(h, rw, wgu, wd, 2, qat=qat))
