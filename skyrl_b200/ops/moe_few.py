@@ -112,6 +112,8 @@ def expert_ffn_few(h: torch.Tensor, w: torch.Tensor, idx: torch.Tensor, wgu: tor
         raise ValueError(f"{what}: weights and ids must be fp32 and int32 [{T}, k] tensors")
     if not idx.is_contiguous() or not w.is_contiguous() or idx.get_device() != dev or w.get_device() != dev:
         raise ValueError(f"{what}: weights and ids must be contiguous and on the rows' device")
+    if w.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() (moe_ffn trains)")
     k = idx.shape[1]
     if k < 1 or T * k > MAX_ENTRIES or E > MAX_EXPERTS or F < 1:
         raise ValueError(f"{what}: {T} x {k} entries over {E} experts are out of range (at most {MAX_ENTRIES} over {MAX_EXPERTS})")

@@ -115,3 +115,12 @@ def test_supports():
     assert moe_few.supports(64, 128, 8, 2048, 768) and moe_few.supports(256, 128, 8, 2048, 768)
     for bad in ((257, 128, 8, 2048, 768), (4, 2000, 8, 64, 64), (4, 64, 17, 64, 64), (4, 4, 5, 64, 64), (4, 8, 2, 60, 64), (4, 8, 2, 64, 60)):
         assert not moe_few.supports(*bad)
+
+
+def test_routing_weights_with_gradients_are_refused():
+    h, rw, wgu, wd = make(3, 4, 2, 16, 8)
+    w, idx = moe_few.route_few(h, rw, 2)
+    with pytest.raises(ValueError, match="gradient"):
+        moe_few.expert_ffn_few(h, w.clone().requires_grad_(), idx, wgu, wd)
+    with torch.no_grad():
+        moe_few.expert_ffn_few(h, w.clone().requires_grad_(), idx, wgu, wd)
