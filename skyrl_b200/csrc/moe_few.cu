@@ -425,11 +425,15 @@ __device__ __forceinline__ Unit unit_at(const Lists& L, int unit) {
 // their sums meet in shared memory at the end of the item.  A warp's share stays in registers, so that wide rows need all
 // eight warps; narrow ones leave groups that hide one another's barriers (gate and up of 64 tokens, 128 experts of
 // 1024 x 512, top 8: 66 us with one group, 51 with two; of 28 tokens, 159 experts of 1288 x 728: 89 and 81).
+// A stage always returns to the group that used it last: the ring's length is a multiple of the blocks that a round of all
+// groups takes.  Copies may land in any order, and a group that met a stage for the first time could find the other group's
+// copy still under way; the parity it waits for would then name the phase before that copy, which is complete, and the wait
+// would end at once.
 // ---------------------------------------------------------------------------
 constexpr int kConsumers = 8;
 constexpr int kConsumerThreads = 32 * kConsumers;
 constexpr int kRingThreads = kConsumerThreads + 32;
-constexpr int kMaxStages = 24;
+constexpr int kMaxStages = 32;
 constexpr int kMaxPiece = 2048;  // columns
 // k steps of 32 columns, at most, of a warp's share: more than twelve spill with 16 rows a unit
 __host__ __device__ constexpr int max_steps(int group) { return group == kConsumers ? kMaxPiece / 32 / kConsumers : 12; }
@@ -907,15 +911,33 @@ down_once_kernel(const __nv_bfloat16* act, const int* idx, const float* w, const
   combine(y, idx, w, out, n0, T, k, E, H, 0, 1);
 }
 
-// Stages of eight rows of K columns in `room` bytes.  A row of more than kMaxPiece columns comes in equal pieces.
-inline Shape ring_shape(int K, size_t room) {
+// The gate and up kernel's ring for rows of K columns beside the lists of n entries over E experts: stages of eight rows
+// (or of pieces of them, equal ones, where a row has more than kMaxPiece columns), and as few warps a group as the columns
+// allow.
+struct RingPlan {
   Shape s;
+  int group;    // warps of a consumer group
+  size_t smem;  // dynamic shared memory
+};
+constexpr size_t kMostSmem = 227 * 1024 - sizeof(Ring) - 128;  // dynamic shared memory that a CTA may have beside its Ring
+inline bool plan_ring(int n, int E, int K, RingPlan& plan) {
+  const size_t fixed = kRedBytes + static_cast<size_t>(lists_bytes(n, E));
+  Shape& s = plan.s;
   s.K = K;
   s.pieces = (K + kMaxPiece - 1) / kMaxPiece;
   s.piece = s.pieces == 1 ? K : ((K + s.pieces - 1) / s.pieces + 31) / 32 * 32;
-  const size_t fit = room / (16 * static_cast<size_t>(s.piece));
-  s.stages = static_cast<int>(fit < kMaxStages ? fit : kMaxStages);
-  return s;
+  const size_t fit = (kMostSmem - fixed) / (16 * static_cast<size_t>(s.piece));
+  const int most = static_cast<int>(fit < kMaxStages ? fit : kMaxStages), steps = (s.piece + 31) / 32;
+  for (plan.group = s.pieces > 1 ? kConsumers : 1; plan.group <= kConsumers; plan.group *= 2) {
+    const int round = 2 * kConsumers / plan.group;  // stages that an item of every group takes
+    if (steps > plan.group * max_steps(plan.group)) continue;
+    // one group meets every stage: any length will do
+    s.stages = plan.group == kConsumers ? most : most / round * round;
+    if (s.stages < round) continue;
+    plan.smem = fixed + static_cast<size_t>(s.stages) * 16 * s.piece;
+    return true;
+  }
+  return false;
 }
 
 template <int kGroup>
@@ -1000,6 +1022,20 @@ int sb_moe_few_route(const void* h, long long h_stride, const void* router, cons
   return cudaGetLastError() == cudaSuccess ? SB_OK : SB_ERR_CUDA;
 }
 
+// The ring that sb_moe_few_experts takes for n = T * k entries over E experts of rows of H columns: stages, pieces a row,
+// columns a piece, consumer groups, bytes of dynamic shared memory.  Host only.
+int sb_moe_few_ring(int n, int E, int H, int* stages, int* pieces, int* piece, int* groups, int* smem) {
+  sb::mf::RingPlan p;
+  if (n <= 0 || n > sb::mf::kMaxEntries || E <= 0 || E > sb::mf::kMaxExperts || H <= 0 || (H & 7)) return SB_ERR_ARG;
+  if (!sb::mf::plan_ring(n, E, H, p)) return SB_ERR_TOO_LARGE;
+  *stages = p.s.stages;
+  *pieces = p.s.pieces;
+  *piece = p.s.piece;
+  *groups = sb::mf::kConsumers / p.group;
+  *smem = static_cast<int>(p.smem);
+  return SB_OK;
+}
+
 // h [T, H], idx int32 / w fp32 [T, k] (idx outside [0, E): the slot contributes nothing), wgu [E, 2F, H], wd [E, H, F];
 // act: [T * k, F] scratch; out [T, H].
 int sb_moe_few_experts(const void* h, long long h_stride, const float* w, const int* idx, const void* wgu, const void* wd,
@@ -1014,19 +1050,14 @@ int sb_moe_few_experts(const void* h, long long h_stride, const float* w, const 
   int* status = sb::device_status_ptr();
   if (!status) return SB_ERR_CUDA;
   const int n = T * k;
-  // what a CTA may have (227 KB) less the row lists and the warps' sums
-  const size_t most = 227 * 1024 - sizeof(sb::mf::Ring) - 128;
-  const size_t lists = sb::mf::lists_bytes(n, E), fixed = sb::mf::kRedBytes + lists;
-  const sb::mf::Shape gu = sb::mf::ring_shape(H, most - fixed);
-  if (gu.stages < 2) return SB_ERR_TOO_LARGE;
-  const size_t smem_gu = fixed + static_cast<size_t>(gu.stages) * 16 * gu.piece;
-  // as few warps a group as the columns allow
-  const int steps = (gu.piece + 31) / 32;
-  const auto launch = gu.pieces > 1 || steps > 4 * sb::mf::max_steps(4) ? sb::mf::launch_gate_up<8>
-                      : steps > 2 * sb::mf::max_steps(2)                ? sb::mf::launch_gate_up<4>
-                      : steps > sb::mf::max_steps(1)                    ? sb::mf::launch_gate_up<2>
-                                                                        : sb::mf::launch_gate_up<1>;
-  cudaError_t e = launch(h, h_stride, idx, wgu, act, T, k, E, H, F, gu, smem_gu, most, status, st);
+  const size_t most = sb::mf::kMostSmem, lists = sb::mf::lists_bytes(n, E);
+  sb::mf::RingPlan gu;
+  if (!sb::mf::plan_ring(n, E, H, gu)) return SB_ERR_TOO_LARGE;
+  const auto launch = gu.group == 8   ? sb::mf::launch_gate_up<8>
+                      : gu.group == 4 ? sb::mf::launch_gate_up<4>
+                      : gu.group == 2 ? sb::mf::launch_gate_up<2>
+                                      : sb::mf::launch_gate_up<1>;
+  cudaError_t e = launch(h, h_stride, idx, wgu, act, T, k, E, H, F, gu.s, gu.smem, most, status, st);
   if (e != cudaSuccess) return SB_ERR_CUDA;
   const size_t once = sb::mf::once_bytes(n, F) + lists;
   if (n <= sb::mf::kOnceUnits && once <= most)
