@@ -476,15 +476,16 @@ __device__ __forceinline__ void group_sync(int group) {
 }
 
 // Fill the stages of one item (called by a whole warp): blocks of rows_a rows at a and rows_b rows at b.  Returns false
-// when a wait gave up.
-__device__ __forceinline__ bool produce_item(Ring& ring, char* buf, const Shape& s, Turn& turn, const __nv_bfloat16* a, int rows_a,
-                                             const __nv_bfloat16* b, int rows_b, int* status) {
+// when a wait gave up.  `filled` counts the stages filled.
+__device__ __forceinline__ bool produce_item(Ring& ring, char* buf, const Shape& s, Turn& turn, long long& filled, const __nv_bfloat16* a,
+                                             int rows_a, const __nv_bfloat16* b, int rows_b, int* status) {
   const int lane = threadIdx.x & 31;
   for (int q = 0; q < s.pieces; ++q)
-    for (int half = 0; half < 2; ++half, turn.step(s.stages)) {
+    for (int half = 0; half < 2; ++half, ++filled, turn.step(s.stages)) {
       const __nv_bfloat16* src = half ? b : a;
       const int rows = half ? rows_b : rows_a;
-      if (!mbar_wait(&ring.empty[turn.stage], turn.parity ^ 1, status, 0x4d01)) return false;
+      // the warp gives up as one: no lane copies to a stage that another did not announce
+      if (!__all_sync(0xffffffffu, mbar_wait(&ring.empty[turn.stage], turn.parity ^ 1, status, 0x4d01))) return false;
       const uint32_t bytes = 2u * min(s.piece, s.K - q * s.piece);
       char* dst = buf + static_cast<size_t>(turn.stage) * 16 * s.piece;
       if (lane == 0) mbar_arrive_expect_tx(&ring.full[turn.stage], bytes * rows);
@@ -530,7 +531,9 @@ __device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red
   Turn turn;
   for (int i = 0; i < 2 * group; ++i) turn.step(s.stages);  // more than one group: rows of one piece
   int r0 = -1;
-  bool ok = true;  // after a wait gave up, the items are run through without waiting: every warp still meets the others
+  // After a wait gave up, the items are run through without waiting: every warp still meets the others.  It gives no stage
+  // back any more, so that none is filled over a copy that has not landed: the producer's wait ends too, as the status is set.
+  bool ok = true;
   float4* sums = red + group * (2 * kGroup * kNt * 32);
   for (int i = group; i < items; i += kGroups) {
     const Unit u = unit_of();
@@ -554,11 +557,11 @@ __device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red
       const int off = g * 2 * s.piece + lo * 64 + 16 * t4;
       const char* top = buf + static_cast<size_t>(turn.stage) * 16 * s.piece + off;
       uint64_t* free_a = &ring.empty[turn.stage];
-      ok = ok && mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d02);
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d02));
       turn.step(s.stages);
       const char* low = buf + static_cast<size_t>(turn.stage) * 16 * s.piece + off;
       uint64_t* free_b = &ring.empty[turn.stage];
-      ok = ok && mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d03);
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&ring.full[turn.stage], turn.parity, status, 0x4d03));
       turn.step(s.stages);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
@@ -575,7 +578,7 @@ __device__ __forceinline__ void consume(Ring& ring, const char* buf, float4* red
         }
       }
       __syncwarp();
-      if (lane == 0) {
+      if (lane == 0 && ok) {
         mbar_arrive(free_a);
         mbar_arrive(free_b);
       }
@@ -609,12 +612,19 @@ __device__ __forceinline__ void ring_init(Ring& ring, int stages, int group_warp
     fence_mbar_init();
   }
 }
-// After a wait gave up: let the copies that are still under way land before the CTA's shared memory is given back.
-__device__ __forceinline__ void ring_drain(Ring& ring, const Shape& s, Turn turn) {
-  for (int i = 0; i < s.stages; ++i, turn.step(s.stages)) {  // from the oldest stage on; a stage never filled waits in vain
-    const unsigned long long t0 = globaltimer_ns();
-    while (!mbar_try_wait(&ring.full[turn.stage], turn.parity ^ 1))
-      if (globaltimer_ns() - t0 > kWaitTimeoutNs / 100) break;
+// The producer's end: copies that are still under way land before the CTA's shared memory is given back.  The consumers
+// wait for them too, but one that gave up does not.  `filled`: stages filled in all, the last of them before `turn`.
+__device__ __forceinline__ void ring_drain(Ring& ring, const Shape& s, Turn turn, long long filled) {
+  Turn oldest;  // of the last s.stages fills
+  if (filled >= s.stages) {
+    oldest = turn;
+    oldest.parity ^= 1;
+  }
+  const int n = filled < s.stages ? static_cast<int>(filled) : s.stages;
+  const unsigned long long t0 = globaltimer_ns();
+  for (int i = 0; i < n; ++i, oldest.step(s.stages)) {
+    while (!mbar_try_wait(&ring.full[oldest.stage], oldest.parity))
+      if (globaltimer_ns() - t0 > kWaitTimeoutNs) break;
   }
 }
 
@@ -640,18 +650,18 @@ gate_up_kernel(const __nv_bfloat16* h, long long h_stride, const int* idx, const
   if (threadIdx.x >= kConsumerThreads) {
     Turn turn;
     int unit = lo / tiles, tile = lo - unit * tiles;
+    long long filled = 0;
+    bool ok = true;
     fence_proxy_async_global();
-    for (int i = lo; i < hi; ++unit, tile = 0) {
+    for (int i = lo; ok && i < hi; ++unit, tile = 0) {
       const Unit u = unit_at(L, unit);
-      for (; tile < tiles && i < hi; ++tile, ++i) {
+      for (; ok && tile < tiles && i < hi; ++tile, ++i) {
         const int f0 = tile * 8, rows = min(8, F - f0);
         const __nv_bfloat16* w = wgu + (static_cast<size_t>(u.e) * 2 * F + f0) * H;
-        if (!produce_item(ring, buf, s, turn, w, rows, w + static_cast<size_t>(F) * H, rows, status)) {
-          ring_drain(ring, s, turn);
-          return;
-        }
+        ok = produce_item(ring, buf, s, turn, filled, w, rows, w + static_cast<size_t>(F) * H, rows, status);
       }
     }
+    ring_drain(ring, s, turn, filled);
     return;
   }
   auto run = [&](auto nt) {
@@ -894,10 +904,12 @@ down_once_kernel(const __nv_bfloat16* act, const int* idx, const float* w, const
   }
   __syncwarp();
   for (int i = warp; i < L.n_units; i += kWarps) {
-    if (!mbar_wait(&full[i], 0, status, 0x4d04)) {  // the copy still lands before the buffer is given back
+    // the warp gives up as one, and its copy still lands before the buffer is given back
+    if (!__all_sync(0xffffffffu, mbar_wait(&full[i], 0, status, 0x4d04))) {
       const unsigned long long t0 = globaltimer_ns();
       while (!mbar_try_wait(&full[i], 0))
-        if (globaltimer_ns() - t0 > kWaitTimeoutNs / 100) break;
+        if (globaltimer_ns() - t0 > kWaitTimeoutNs) break;
+      __syncwarp();
       continue;
     }
     const Unit u = unit_at(L, i);
