@@ -40,9 +40,9 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 // Router.  A cluster of eight CTAs takes eight tokens and an eighth of the experts each, 16 experts at a time; the CTA's
 // warps split the columns, and the logits of token i meet in CTA i's shared memory.  Products of bf16 are exact in the
 // matrix unit; its fp32 sums are taken out every 32 columns and carried on in two fp32 words, and where the order still
-// hangs on their error (one row in 700 at 128 experts) the logits in question are summed again in fp64: experts are ordered
-// by the values, equal ones by their number.  128 experts, rows of 2048: 4.8 us for one token, 5.4 for 64, of which 0.3 are
-// that check; a row with logits in question takes 3 to 4 more.
+// hangs on their error (one row in 140 at 128 experts) the logits in question are summed again in fp64: experts are ordered
+// by the values, equal ones by their number.  128 experts, rows of 2048: 4.6 us for one token, 4.9 for 64, of which 0.3 are
+// that check; a call with a row whose logits are in question takes 3 more.
 // The k largest are found by rank, the number of experts that come before one: all are compared with one another at once,
 // where k rounds of a maximum would wait for one another.  Beyond kRankGroup experts, passes over groups leave k
 // candidates each, and a last pass ranks those.
@@ -51,10 +51,11 @@ constexpr int kCluster = 8;  // CTAs, and tokens
 constexpr int kRouteThreads = 256;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRankGroup = 128;  // entries ranked in a pass, two lanes each
-// Logits that lie closer than this share of the largest sum of magnitudes are compared in fp64.  A product of 16 columns
-// has 17 addends, each cut off at 2^-24 of the largest, which is at most about a third of their sum in rows of a model:
-// twice 17/3 * 2^-24 for two logits, just under 2^-20.
-constexpr double kLogitError = 1.0 / (1 << 20);
+// Logits that lie closer than this share of the largest sum of magnitudes are compared in fp64.  Each of the 16 addends of
+// a product is cut off at 2^-24 of the largest one, its result at 2^-23, and two results are added in fp32: 19 * 2^-24 of
+// the 32 columns' sum of magnitudes, however one of them dominates.  Two logits: 38 * 2^-24, below 2^-18.  (A product that
+// starts from another's result cuts off at that: such a chain would need twice as much.)
+constexpr double kLogitError = 1.0 / (1 << 18);
 constexpr int kExactBatch = 4;
 
 // Order-preserving key of a logit, unique: the lowest ten bits hold the expert, the lower one first among equals.  A NaN
@@ -127,16 +128,16 @@ route_kernel(const __nv_bfloat16* __restrict__ h, long long h_stride, const __nv
       }
 #pragma unroll
       for (int j = 0; j < kUnroll; ++j) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        float d[4] = {0.f, 0.f, 0.f, 0.f}, d2[4] = {0.f, 0.f, 0.f, 0.f};
         mma_bf16(d, a[j].x, b[j].x, a[j].y, b[j].y, v[j].x, v[j].y);
-        mma_bf16(d, a[j].z, b[j].z, a[j].w, b[j].w, v[j].z, v[j].w);
+        mma_bf16(d2, a[j].z, b[j].z, a[j].w, b[j].w, v[j].z, v[j].w);
         constexpr uint32_t kAbs = 0x7fff7fffu;
         mma_bf16(mag, a[j].x & kAbs, b[j].x & kAbs, a[j].y & kAbs, b[j].y & kAbs, v[j].x & kAbs, v[j].y & kAbs);
         mma_bf16(mag, a[j].z & kAbs, b[j].z & kAbs, a[j].w & kAbs, b[j].w & kAbs, v[j].z & kAbs, v[j].w & kAbs);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float sum = hi[c] + d[c], back = sum - hi[c];
-          lo[c] += (hi[c] - (sum - back)) + (d[c] - back);  // what the addition rounded away
+          const float both = d[c] + d2[c], sum = hi[c] + both, back = sum - hi[c];
+          lo[c] += (hi[c] - (sum - back)) + (both - back);  // what the addition rounded away
           hi[c] = sum;
         }
       }
