@@ -861,15 +861,15 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     }
   }
   if (lane == 0) {
-    if (!ok) {  // loads that are still under way land before the buffers are given back
-      for (int j = i + 1; j < min(count, i + kStages - 1); ++j) {
+    if (!ok) {  // loads that are still under way, piece i's and those behind it, land before the buffers are given back
+      const unsigned long long t0 = globaltimer_ns();
+      for (int j = i; j < min(count, i + kStages - 1); ++j) {
+        while (!mbar_try_wait(&bar[stage], parity))
+          if (globaltimer_ns() - t0 > kWaitTimeoutNs) break;
         if (++stage == kStages) {
           stage = 0;
           parity ^= 1;
         }
-        const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(&bar[stage], parity))
-          if (globaltimer_ns() - t0 > kWaitTimeoutNs) break;
       }
     }
     tma_store_wait_read<0>();  // the buffers have been read; the writes end with the kernel

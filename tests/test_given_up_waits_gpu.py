@@ -9,7 +9,7 @@ import pytest
 import torch
 from test_moe_few_cpu import make
 
-from skyrl_b200.ops import _lib, moe_few
+from skyrl_b200.ops import _lib, elementwise, moe_few, rotary
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -48,4 +48,30 @@ def test_experts(status, T, E, k, H, F):
     assert torch.equal(beside[0], w) and torch.equal(beside[1], idx)
     assert _lib.status_read_clear() == 0x901  # the barrier's code: the first wait that gave up
     assert torch.equal(moe_few.expert_ffn_few(h, w, idx, wgu, wd), want)
+    assert _lib.status_read_clear() == 0
+
+
+@pytest.mark.parametrize("D,R,dtype", [(128, 128, BF), (80, 20, torch.float16), (64, 64, torch.float32)])
+def test_row_pipeline(status, D, R, dtype):
+    T, nq, nkv = 8192, 8, 2
+    g = torch.Generator(device="cuda").manual_seed(D)
+    x, dy = (torch.randn(T, (nq + 2 * nkv) * D, generator=g, device="cuda").to(dtype) for _ in range(2))
+    qw, kw = (torch.rand(D, generator=g, device="cuda").to(dtype) + 0.5 for _ in range(2))
+    pos = torch.arange(T, device="cuda", dtype=torch.int32)
+    table = elementwise.build_rope_table(T, R, 1e4, "cuda")
+
+    def step():
+        a = [t.clone().requires_grad_() for t in (x, qw, kw)]
+        y = rotary.qk_norm_rope(*a, pos, table, nq, nkv, D, 1e-6)
+        return [y.detach(), *torch.autograd.grad(y, a, dy)]
+
+    want = step()
+    status()
+    for _ in range(10):
+        step()
+        beside = rotary.rotary(x[:64], pos[:64], table, nq + nkv, D)  # too few rows for the pipeline
+    torch.cuda.synchronize()
+    assert _lib.status_read_clear() == 0x901
+    assert torch.equal(beside, rotary.rotary(x, pos, table, nq + nkv, D)[:64])
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
     assert _lib.status_read_clear() == 0
