@@ -351,8 +351,10 @@ class CausalLM(nn.Module):
         elif a.num_experts:
             from .moe import moe_ffn
 
+            # with and without gradients alike: a forward that scores tokens matches the one that trains on them
             d = moe_ffn(h, self.p(pre + "router"), self.p(pre + "experts_wgu"), self.p(pre + "experts_wd"),
-                        a.num_experts_per_tok, a.norm_topk_prob, layer=i, qat=getattr(self, "fake_int4_qat", None))
+                        a.num_experts_per_tok, a.norm_topk_prob, layer=i, qat=getattr(self, "fake_int4_qat", None),
+                        few_tokens=kv_sink is not None)
         else:
             d = gemm.swiglu_mlp(h, self.p(pre + "wgu"), self.p(pre + "wd"))
         return x, d

@@ -16,9 +16,10 @@ from ..ops import gemm  # noqa: F401
 from ..ops import grouped_gemm as gg
 from ..ops import moe_few
 
-# Up to this many rows an expert in the mean, and without gradients, the layer runs on ``ops/moe_few.py``.  Layer times
-# there / through the grouped GEMMs in us: 128 experts of 2048 x 768, top 8: 191 / 362 at 64 tokens (4 rows), 326 / 368 at
-# 256 (16 rows); 8 experts of 2048 x 4096, top 2: 115 / 164 at 64 tokens (16 rows), 178 / 154 at 128 (32 rows).
+# Up to this many rows an expert in the mean, and without gradients, the layer runs on ``ops/moe_few.py`` unless the caller
+# rules it out.  Layer times there / through the grouped GEMMs in us: 128 experts of 2048 x 768, top 8: 191 / 362 at 64
+# tokens (4 rows), 326 / 368 at 256 (16 rows); 8 experts of 2048 x 4096, top 2: 115 / 164 at 64 tokens (16 rows), 178 / 154
+# at 128 (32 rows).
 FEW_ROWS = 16
 
 
@@ -87,14 +88,16 @@ def _takes_few(h, router_w, wgu, wd, top_k) -> bool:
 
 def moe_ffn(h: torch.Tensor, router_w: torch.Tensor, wgu: torch.Tensor, wd: torch.Tensor, top_k: int,
             norm_topk_prob: bool = True, routed_indices: torch.Tensor | None = None, layer: int | None = None, qat=None,
-            live: torch.Tensor | None = None) -> torch.Tensor:
+            live: torch.Tensor | None = None, few_tokens: bool = True) -> torch.Tensor:
     """``h``: [T, H]; ``wgu``: [E, 2F, H]; ``wd``: [E, H, F].  ``routed_indices`` replays rollout-time routing;
     with ``layer`` given, an active ``router_replay`` context records or overrides the choice.  ``live`` ([T] int32):
-    rows whose result is not used where it is 0; on the path for few tokens they read no expert and come out zero."""
+    rows whose result is not used where it is 0; on the path for few tokens they read no expert and come out zero.
+    ``few_tokens=False`` keeps a small batch on the grouped GEMMs.  The two paths round at different places and may order
+    near ties differently, so log-probabilities that meet a training forward's are computed that way."""
     T, H = h.shape
     E = wgu.shape[0]
     quantised = qat is not None and qat.enabled and torch.is_grad_enabled()
-    few = not quantised and _takes_few(h, router_w, wgu, wd, top_k)
+    few = few_tokens and not quantised and _takes_few(h, router_w, wgu, wd, top_k)
     if few:
         w, idx = moe_few.route_few(h, router_w, top_k, norm_topk_prob, live=live)
     else:
