@@ -81,7 +81,7 @@ def _takes_few(h, router_w, wgu, wd, top_k) -> bool:
         return False
     if torch.is_grad_enabled() and any(t.requires_grad for t in (h, router_w, wgu, wd)):
         return False
-    if not all(t.dtype == h.dtype and t.is_contiguous() for t in (router_w, wgu, wd)):
+    if not all(t.dtype == h.dtype and t.is_contiguous() and t.data_ptr() % 16 == 0 for t in (router_w, wgu, wd)):
         return False
     return moe_few.supports(h.shape[0], wgu.shape[0], top_k, h.shape[1], wd.shape[2])
 

@@ -36,9 +36,17 @@ def supports(T: int, num_experts: int, top_k: int, H: int, F: int) -> bool:
             and H % 8 == 0 and F % 8 == 0)
 
 
-def _rows(h: torch.Tensor) -> torch.Tensor:
-    ok = h.stride(1) == 1 and (h.stride(0) % 8 == 0 or h.shape[0] == 1) and h.stride(0) >= h.shape[1] and h.data_ptr() % 16 == 0
-    return h if ok else h.contiguous()
+def _aligned(*ts: torch.Tensor) -> bool:
+    return all(t.data_ptr() % 16 == 0 for t in ts)
+
+
+def _rows(h: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """Rows that the kernels can read 16 bytes at a time, and their stride (of a single row: any that fits)."""
+    T, H = h.shape
+    ok = h.stride(1) == 1 and (T == 1 or (h.stride(0) % 8 == 0 and h.stride(0) >= H)) and _aligned(h)
+    if not ok:
+        h = torch.empty_like(h, memory_format=torch.contiguous_format).copy_(h)
+    return h, h.stride(0) if T > 1 else H
 
 
 def _check_common(what, h, a, b):
@@ -51,6 +59,8 @@ def _check_common(what, h, a, b):
         raise ValueError(f"{what}: weights must be contiguous")
     if dev >= 0 and (dt != torch.bfloat16 or h.shape[1] % 8):
         raise ValueError(f"{what}: CUDA rows must be bf16 with a width that is a multiple of 8, got {dt} [{h.shape[1]}]")
+    if dev >= 0 and not _aligned(a, b):
+        raise ValueError(f"{what}: weights must start on a 16-byte boundary")
     return dev
 
 
@@ -89,8 +99,8 @@ def route_few(h: torch.Tensor, router_w: torch.Tensor, top_k: int, norm_topk_pro
     idx = torch.empty_like(w, dtype=torch.int32)
     if T == 0:
         return w, idx
-    h = _rows(h)
-    code = _lib.call_on(dev, _k().sb_moe_few_route, h.data_ptr(), h.stride(0), router_w.data_ptr(),
+    h, stride = _rows(h)
+    code = _lib.call_on(dev, _k().sb_moe_few_route, h.data_ptr(), stride, router_w.data_ptr(),
                         None if live is None else live.data_ptr(), w.data_ptr(), idx.data_ptr(), T, E, H, top_k,
                         bool(norm_topk_prob))
     _lib.check(code, "sb_moe_few_route")
@@ -136,9 +146,9 @@ def expert_ffn_few(h: torch.Tensor, w: torch.Tensor, idx: torch.Tensor, wgu: tor
     out = torch.empty_like(h, memory_format=torch.contiguous_format)
     if T == 0:
         return out
-    h = _rows(h)
+    h, stride = _rows(h)
     act = h.new_empty(T * k * F)
-    code = _lib.call_on(dev, _k().sb_moe_few_experts, h.data_ptr(), h.stride(0), w.data_ptr(), idx.data_ptr(), wgu.data_ptr(),
+    code = _lib.call_on(dev, _k().sb_moe_few_experts, h.data_ptr(), stride, w.data_ptr(), idx.data_ptr(), wgu.data_ptr(),
                         wd.data_ptr(), act.data_ptr(), out.data_ptr(), T, k, E, H, F)
     _lib.check(code, "sb_moe_few_experts")
     return out
