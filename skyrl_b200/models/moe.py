@@ -105,7 +105,8 @@ def moe_ffn(h: torch.Tensor, router_w: torch.Tensor, wgu: torch.Tensor, wd: torc
     if layer is not None and routed_indices is None:
         from . import router_replay
 
-        routed_indices = router_replay.on_route(layer, idx.long())
+        if router_replay.active():  # else no cast between the routing kernel and those that start beside its end
+            routed_indices = router_replay.on_route(layer, idx.long())
     if routed_indices is not None:
         probs = torch.softmax(h.float() @ router_w.float().t(), dim=-1)
         idx = routed_indices.long()
