@@ -93,6 +93,9 @@ class ModelArgs:
         rope = dict(cfg.get("rope_parameters") or cfg.get("rope_scaling") or {})
         theta = cfg.get("rope_theta", rope.pop("rope_theta", 10000.0))
         partial = cfg.get("partial_rotary_factor", rope.pop("partial_rotary_factor", 1.0)) or 1.0
+        if float(partial) != 1.0 and "rope_interleaved" not in cfg:  # no key of a checkpoint tells the two layouts apart
+            logger.warning("heads are rotated in part (%s), pairs taken from the two halves of that part; 'rope_interleaved': true "
+                           "in the configuration rotates neighbouring elements instead", partial)
         kind = rope.get("rope_type") or rope.get("type") or "default"
         if kind not in ("default", "linear", "llama3", "yarn"):
             logger.warning("rope scaling '%s' is not supported: positions are not scaled", kind)
@@ -132,8 +135,8 @@ class ModelArgs:
             cfg["rope_scaling"] = dict(self.rope_scaling)
         if self.partial_rotary_factor != 1.0:
             cfg["partial_rotary_factor"] = self.partial_rotary_factor
-        if self.rope_interleaved:
-            cfg["rope_interleaved"] = True
+        if self.rope_interleaved or self.partial_rotary_factor != 1.0:
+            cfg["rope_interleaved"] = self.rope_interleaved
         if self.attention_sinks:
             cfg["attention_sinks"] = True
         if self.num_experts:
