@@ -88,7 +88,7 @@ def _share_memory(x: torch.Tensor, out: torch.Tensor) -> bool:
     if x.dim() == 3:
         return x.data_ptr() < end(out) and out.data_ptr() < end(x[-1])
     if out.data_ptr() == x.data_ptr():
-        return x.shape[0] > 1 and out.stride() != x.stride()
+        return not _is_row_major(x) or (x.shape[0] > 1 and out.stride(0) != x.stride(0))
     if not _is_row_major(x) or out.data_ptr() >= end(x) or x.data_ptr() >= end(out):  # the first: read from a copy
         return False
     if x.shape[0] == 1 or out.stride(0) != x.stride(0):
