@@ -663,7 +663,10 @@ constexpr int kRowWarps = 16;
 enum Mode { kRotate, kNormRotate, kNormBack };
 
 // kFine: the rotated width is a multiple of 4, not of 8, so that a lane may own two pairs that rotate and two that do not.
-template <typename T, bool kInter, bool kFine, Mode kMode>
+// kPart (with norms): heads are rotated in part.  Elements that do not rotate go through times 1 plus 0 times their
+// neighbour; where that may be infinite, which shows in the head's sum, they are made again without it.  16384 rows of 32 + 4
+// + 4 heads of 128, with kPart / without: forward 62 / 59 us, backward 94 / 89.
+template <typename T, bool kInter, bool kFine, Mode kMode, bool kPart>
 __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, int piece_bytes, int* status) {
   constexpr bool kBack = kMode == kNormBack;
   extern __shared__ __align__(128) char smem[];
@@ -737,6 +740,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
   int stage = 0;
   uint32_t parity = 0;
   bool ok = true;
+  float least = 1.f;  // of a piece's factors r: 0 where a head's sum is infinite
   int i = 0;
   for (; i < count; ++i) {
     // forward: a -> a c - b s, b -> b c + a s; backwards with -s
@@ -801,6 +805,16 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
             if (kBack) m += __shfl_xor_sync(0xffffffffu, m, 1 << o);
           }
           r = rsqrtf(r * inv_d + a.eps);
+          if (kPart && kBack && !rot2 && !(fabsf(m) < __int_as_float(0x7f800000))) {
+            const Pairs u = get_pairs<T, kInter, kFine>(row, at);
+            if (!rot) {
+              v.a[0] = u.a[0];
+              v.b[0] = u.b[0];
+            }
+            v.a[1] = u.a[1];
+            v.b[1] = u.b[1];
+          }
+          if (kPart && !kBack) least = fminf(least, r);
         }
         const f2 r2 = pack2(r, r);
         __syncwarp();  // every lane has read its elements before one that goes along with it writes them
@@ -832,6 +846,23 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) rows_kernel(const Args a, i
     };
     heads(h0, min(h1, a.nq), static_cast<const T*>(a.qw), acc_q);
     heads(max(h0, a.nq), min(h1, turned), static_cast<const T*>(a.kw), acc_k);
+    if (kPart && !kBack && __any_sync(0xffffffffu, least == 0.f)) {  // from the row, whose own memory is not written yet
+      least = 1.f;
+      __syncwarp();  // every lane has written its elements
+      for (int h = h0 + sub; h - sub < min(h1, turned); h += hpw) {
+        const bool on = live && h < min(h1, turned);
+        const int hh = on ? h : h0;
+        const T* src = static_cast<const T*>(a.src) + static_cast<size_t>(t) * a.src_stride + hh * a.D;
+        const T* w = static_cast<const T*>(hh < a.nq ? a.qw : a.kw);
+        float ss = 0.f;
+        if (on)
+          for (int e = c * 8; e < c * 8 + 8; ++e) ss += to_f(src[e]) * to_f(src[e]);
+        ss = group_sum(ss, a.log_group);
+        if (!on || rsqrtf(ss * inv_d + a.eps) != 0.f) continue;
+        T* row = reinterpret_cast<T*>(piece) + (h - h0) * a.D;
+        for (int e = max(a.R, c * 8); e < c * 8 + 8; ++e) row[e] = from_f<T>(to_f(src[e]) * 0.f * to_f(w[e]));
+      }
+    }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
@@ -1099,7 +1130,7 @@ int log2_ceil(int v) {
 // The row pipeline: heads of a piece so that a CTA's buffers fill at most kRowSmem.
 constexpr int kRowSmem = 200 * 1024;
 
-template <typename T, bool kInter, bool kFine, Mode kMode>
+template <typename T, bool kInter, bool kFine, Mode kMode, bool kPart>
 cudaError_t launch_rows_as(Args a, int ctas, cudaStream_t st) {
   const int head = a.D * static_cast<int>(sizeof(T)), per_head = kRowWarps * kStages * head * (kMode == kNormBack ? 2 : 1);
   int block = kRowSmem / per_head;  // as large as the buffers allow, and alike
@@ -1111,19 +1142,22 @@ cudaError_t launch_rows_as(Args a, int ctas, cudaStream_t st) {
   static bool attr_dev[64] = {};
   bool& attr = attr_dev[device_index()];
   if (!attr) {
-    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, kInter, kFine, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
+    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, kInter, kFine, kMode, kPart>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem);
     if (e != cudaSuccess) return e;
     attr = true;
   }
   int* status = device_status_ptr();
   if (!status) return cudaErrorUnknown;
   a.log_group = log2_ceil(a.D / 8);
-  return launch_pdl(rows_kernel<T, kInter, kFine, kMode>, dim3(ctas), dim3(kRowWarps * 32), smem, st, a, block * head, status);
+  return launch_pdl(rows_kernel<T, kInter, kFine, kMode, kPart>, dim3(ctas), dim3(kRowWarps * 32), smem, st, a, block * head, status);
 }
 
 template <typename T, bool kInter, Mode kMode>
 cudaError_t launch_rows(const Args& a, int ctas, cudaStream_t st) {
-  return a.R % 8 ? launch_rows_as<T, kInter, true, kMode>(a, ctas, st) : launch_rows_as<T, kInter, false, kMode>(a, ctas, st);
+  constexpr bool kNorm = kMode != kRotate;
+  if (a.R % 8) return launch_rows_as<T, kInter, true, kMode, kNorm>(a, ctas, st);
+  return kNorm && a.R < a.D ? launch_rows_as<T, kInter, false, kMode, kNorm>(a, ctas, st)
+                            : launch_rows_as<T, kInter, false, kMode, false>(a, ctas, st);
 }
 
 // From how many bytes of rows on the pipeline is taken.  Below, its start (4 us against 2) costs more than it gains, and
