@@ -4,6 +4,8 @@
     python -m skyrl_b200.benchmarks.bench_kernels --which decode_attn --seqs 64 --ctx 1024
     python -m skyrl_b200.benchmarks.bench_kernels --which attn --seqs 8 --seqlen 2048
     python -m skyrl_b200.benchmarks.bench_kernels --which lmhead --tokens 4096
+    python -m skyrl_b200.benchmarks.bench_kernels --which decode_step --layers 4 --seqs 64     # head norms, experts
+    python -m skyrl_b200.benchmarks.bench_kernels --which norm_layers --layers 4 --tokens 8192
 
 Peaks default to the values measured on the B200 pool (copy bandwidth 6543.4 GB/s, bf16 GEMM 1668.8 TFLOP/s burst /
 1376.9 sustained) and can be overridden with --hbm-gbs / --peak-tflops.
@@ -127,14 +129,51 @@ def _bench_lmhead(a) -> dict:
     return res
 
 
+def _bench_norm_model(a):
+    """A few layers of the 30B-A3B architecture (per-head norms): one replayed decode step of ``--seqs`` sequences with its
+    experts, or forward and backward of dense layers over ``--tokens`` tokens."""
+    import dataclasses
+
+    from skyrl_b200.engine.llm_engine import EngineConfig, LLMEngine, SamplingParams
+    from skyrl_b200.models.decoder import PRESETS, CausalLM
+
+    args = dataclasses.replace(PRESETS["qwen3-30b-a3b"], num_layers=a.layers)
+    if a.which == "norm_layers":
+        args = dataclasses.replace(args, num_experts=0, intermediate_size=6144)
+    m = CausalLM(args, device="cuda", dtype=torch.bfloat16, seed=None)
+    m.flat_params.normal_(0, 0.02)
+    with torch.no_grad():
+        for name, p in m.named_flat_views():
+            if name.endswith(("ln1", "ln2", "q_norm", "k_norm", "final_norm")):
+                p.fill_(1.0)
+    g = torch.Generator().manual_seed(0)
+    if a.which == "norm_layers":
+        ids = torch.randint(4, 1000, (a.tokens,), generator=g).cuda()
+        pos = (torch.arange(a.tokens, device="cuda") % 1024).to(torch.int32)
+        cu = torch.tensor([*range(0, a.tokens, 1024), a.tokens], device="cuda", dtype=torch.int32)
+        m.attach_main_grad(torch.zeros(m.flat_numel, device="cuda"))
+        ms = timeit(lambda: m.token_logprobs(m(ids, pos, cu, 1024), ids)[0].sum().backward(), a.iters)
+        return {"layers": a.layers, "tokens": a.tokens, "fwd_bwd_ms": ms}
+    size = 8 if a.seqs <= 8 else a.seqs  # sequences of the captured step; the others are idle
+    eng = LLMEngine(m, EngineConfig(block_size=32, max_num_seqs=size, max_model_len=1024, num_blocks=32 * size + 64,
+                                    graph_batch_sizes=(size,)))
+    prompts = [torch.randint(4, 1000, (500,), generator=g).tolist() for _ in range(a.seqs)]
+    eng.generate(prompts, SamplingParams(max_tokens=8, temperature=0.0, ignore_eos=True))
+    for i, p in enumerate(prompts):
+        eng.add_request(str(i), p, SamplingParams(max_tokens=400, temperature=0.0, ignore_eos=True))
+    eng.step()
+    return {"layers": a.layers, "seqs": a.seqs, "step_us": 1e3 * timeit(eng._graphs[size].replay, a.iters)}
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("--impl", default="ours", choices=["ours", "reference", "both"], help="lmhead: which implementation to time")
     ap.add_argument("--vocab", type=int, default=151936)
     ap.add_argument("--hidden-lm", type=int, default=1536)
     ap.add_argument("--which", default="gemm", choices=["gemm", "decode_attn", "attn", "lmhead", "tp_gather", "tp_scatter", "moe", "elementwise", "relayout",
-                             "decode_block"])
-    ap.add_argument("--layers", type=int, default=8, help="relayout: decoder layers of the Qwen2.5-1.5B-shaped source model")
+                             "decode_block", "decode_step", "norm_layers"])
+    ap.add_argument("--layers", type=int, default=8, help="relayout: decoder layers of the Qwen2.5-1.5B-shaped source model; "
+                    "decode_step, norm_layers: layers of the 30B-A3B-shaped model")
     ap.add_argument("--experts", type=int, default=128)
     ap.add_argument("--topk", type=int, default=8)
     ap.add_argument("--hidden", type=int, default=2048)
@@ -341,6 +380,7 @@ def main() -> None:
         out.update(tokens=T, rows=rows)
     elif a.which == "moe":
         # one mixture-of-experts FFN layer (router, grouped gate/up GEMM, SwiGLU, grouped down GEMM, weighted combine)
+        from skyrl_b200.models import moe
         from skyrl_b200.models.moe import moe_ffn
         from skyrl_b200.ops import grouped_gemm as gg
 
@@ -350,7 +390,9 @@ def main() -> None:
         wgu = (torch.randn(E, 2 * F, H, device="cuda") * 0.02).to(torch.bfloat16)
         wd = (torch.randn(E, H, F, device="cuda") * 0.02).to(torch.bfloat16)
         with torch.no_grad():
-            ms_layer = timeit(lambda: moe_ffn(h, rt, wgu, wd, k, True), a.iters)
+            ms_layer = timeit(lambda: moe_ffn(h, rt, wgu, wd, k, True, few_tokens=False), a.iters)
+            if moe._takes_few(h, rt, wgu, wd, k):
+                out["few_tokens_layer_fwd_ms"] = timeit(lambda: moe_ffn(h, rt, wgu, wd, k, True), a.iters)
             ids = torch.randint(0, E, (T * k,), device="cuda")
             plan = gg.plan_groups(ids, E)
             x = torch.zeros((plan.m_cap, H), **bf)
@@ -361,6 +403,8 @@ def main() -> None:
         out.update(tokens=T, hidden=H, experts=E, ffn=F, topk=k, padded_rows=plan.m_cap, layer_fwd_ms=ms_layer,
                    gate_up_ms=ms_gu, gate_up_tflops=fl_gu / ms_gu / 1e9, down_ms=ms_dn, down_tflops=fl_dn / ms_dn / 1e9,
                    layer_tflops=(fl_gu + fl_dn) / ms_layer / 1e9)
+    elif a.which in ("decode_step", "norm_layers"):
+        out.update(_bench_norm_model(a))
     else:
         out.update(_bench_lmhead(a))
     print(json.dumps(out))
