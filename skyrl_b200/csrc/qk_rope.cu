@@ -37,7 +37,7 @@ struct Args {
   long long src_stride, x_stride, dst_stride, part_stride;
   long long n_slots;
   int n_part, max_pos, T, nq, nk, heads, store_heads, D, R;
-  int log_group;         // lanes of a head: 1 << log_group >= D / 16
+  int log_group;         // lanes of a head: 1 << log_group >= D / 16 (fwd_kernel, bwd_kernel) or D / 8
   int blocks_per_row;    // head blocks a token's heads are split into
   float eps, sign;
 };
@@ -537,11 +537,6 @@ __device__ __forceinline__ void put_pairs(T* p, const Spot& at, const Pairs& v) 
   }
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
 }

@@ -18,8 +18,8 @@ from ..ops import moe_few
 
 # Up to this many rows an expert in the mean, and without gradients, the layer runs on ``ops/moe_few.py`` unless the caller
 # rules it out.  Layer times there / through the grouped GEMMs in us: 128 experts of 2048 x 768, top 8: 191 / 362 at 64
-# tokens (4 rows), 326 / 368 at 256 (16 rows); 8 experts of 2048 x 4096, top 2: 115 / 164 at 64 tokens (16 rows), 178 / 154
-# at 128 (32 rows).
+# tokens (4 rows), 342 / 369 at 256 (16 rows); 8 experts of 2048 x 4096, top 2: 114 / 164 at 64 tokens (16 rows), 178 / 154
+# at 128 (32 rows).  Narrow layers at 16 rows: 104 experts of 552 x 560, top 7: 113 / 140; 64 of 256 x 256, top 4: 52 / 58.
 FEW_ROWS = 16
 
 
