@@ -165,23 +165,26 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None)
     return stretch * inv / factor + (1.0 - stretch) * inv, float(gain)
 
 
-_TABLE_ROWS = 8192  # positions whose angles are formed at a time
+_TABLE_ANGLES = 1 << 21  # formed at a time
 
 
 def build_rope_table(max_pos: int, head_dim: int, theta: float, device, scaling: dict | None = None) -> torch.Tensor:
     """[max_pos, head_dim] fp32: cos in the first half of each row, sin in the second.  For heads that are rotated in
     part, ``head_dim`` is the rotated width.  ``scaling``: see ``rope_frequencies``.  Angles are formed in fp64: at
     position 131072 an fp32 angle would already be off by 2^-8.  They are formed in pieces: beside the table, which may be
-    built when a cache has filled the device, they take a few MB."""
+    built when a cache has filled the device, they take two times 16 MB."""
     inv, gain = rope_frequencies(head_dim, theta, scaling)
     inv = inv.to(device)
     half = inv.numel()
     out = torch.empty((max_pos, 2 * half), device=device, dtype=torch.float32)
-    for lo in range(0, max_pos, _TABLE_ROWS):
-        rows = out[lo : lo + _TABLE_ROWS]
+    step = max(1, _TABLE_ANGLES // half)
+    for lo in range(0, max_pos, step):
+        rows = out[lo : lo + step]
         ang = torch.arange(lo, lo + rows.shape[0], dtype=torch.float64, device=device)[:, None] * inv[None, :]
         for part, fn in ((rows[:, :half], torch.cos), (rows[:, half:], torch.sin)):
-            part.copy_(fn(ang) if gain == 1.0 else fn(ang) * gain)
+            v = fn(ang)
+            part.copy_(v if gain == 1.0 else v.mul_(gain))
+            del v
     return out
 
 

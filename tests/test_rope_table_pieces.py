@@ -19,7 +19,7 @@ def check(device, max_pos, R, scaling):
     assert torch.equal(got, at_once(max_pos, R, 1e4, device, scaling))
 
 
-SIZES = [(1, 2), (8191, 20), (8192, 64), (8193, 128), (40000, 6)]
+SIZES = [(1, 2), (8191, 20), (32768, 128), (32769, 128), (65535, 128), (700000, 6)]
 
 
 @pytest.mark.parametrize("max_pos,R", SIZES)
@@ -45,5 +45,5 @@ def test_memory_beside_the_table(scaling):
     torch.cuda.reset_peak_memory_stats()
     table = ew.build_rope_table(262144, 128, 1e4, "cuda", scaling=scaling)
     beside = torch.cuda.max_memory_allocated() - before - table.numel() * 4
-    # angles, cosines and their scaled copy of 8192 positions in 64 bits, two at a time of 4 MB each, and the positions
-    assert beside <= 24 << 20
+    # angles and cosines (or sines) of 32768 positions in 64 bits, 16 MB each, the positions and the allocator's rounding
+    assert beside <= 36 << 20
