@@ -11,8 +11,9 @@
 // used as the fragments of two products whose k order is permuted the same way in both operands, which a sum over k does
 // not see.  Gate and up weights come through a ring of bulk copies in shared memory, down weights straight from global
 // memory into registers.  Every result is summed in a fixed order, without atomics on floats.
-// 128 experts of 2048 x 768, top 8, bf16, all three launches: 190 us for 64 tokens (124 gate and up, 64 down; 96% of the
-// measured copy bandwidth), 91 for nine, 24 for one, of which 12 are its weights and the rest starts and routing.
+// 128 experts of 2048 x 768, top 8, bf16, all three launches replayed one behind the other, without a profiler: 185 to 190 us
+// for 64 tokens, 97 to 99% of the measured copy bandwidth over the whole layer (alone, gate and up take 120 to 124 and down
+// 64), 91 for nine, 25 for one, of which 12 are its weights and the rest starts and routing.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -424,8 +425,9 @@ __device__ __forceinline__ Unit unit_at(const Lists& L, int unit) {
 // cycles whatever its size: rows of 1.5 KB one by one came at 4.8 TB/s, blocks of 16 to 32 KB come at 6.7 to 6.9.
 // The consumers are groups of kGroup warps; each group takes the next item on, its warps a share of the columns each, and
 // their sums meet in shared memory at the end of the item.  A warp's share stays in registers, so that wide rows need all
-// eight warps; narrow ones leave groups that hide one another's barriers (gate and up of 64 tokens, 128 experts of
-// 1024 x 512, top 8: 66 us with one group, 51 with two; of 28 tokens, 159 experts of 1288 x 728: 89 and 81).
+// eight warps; narrow ones leave groups that hide one another's barriers (gate, up and down of 64 tokens, 128 experts of
+// 1024 x 512, top 8: 89 us with one group, 74 with two; of 28 tokens, 159 experts of 1288 x 728: 133 and 120; of 64 tokens,
+// 128 experts of 256 x 256: 35 with one, 31 with eight).
 // A stage always returns to the group that used it last: the ring's length is a multiple of the blocks that a round of all
 // groups takes.  Copies may land in any order, and a group that met a stage for the first time could find the other group's
 // copy still under way; the parity it waits for would then name the phase before that copy, which is complete, and the wait
