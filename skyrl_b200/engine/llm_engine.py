@@ -187,6 +187,7 @@ class LLMEngine:
         self.eos_token_ids = list(eos_token_ids)
         a = model.args
         c = self.cfg
+        model.rope_table(self.device, c.max_model_len)  # before any graph reads it and before the cache fills the device
         self.max_blocks_per_seq = (c.max_model_len + c.block_size - 1) // c.block_size
         self.num_blocks = c.num_blocks or self._derive_num_blocks()
         self.rt = _rt()

@@ -103,7 +103,7 @@ class TPEngineModel(CausalLM):
         pre = f"layers.{i}."
         x, h = ew.add_rmsnorm(x, delta, self.p(pre + "ln1"), a.rms_norm_eps)
         qkv = gemm.linear(h, self.p(pre + "wqkv"), self._p.get(pre + "bqkv"))
-        qkv = self._rotate(i, qkv, pos, kv_sink)
+        qkv = self._rotate(i, qkv, pos, kv_sink, max_seqlen=max_seqlen)
         if attn_fn is not None:
             att = attn_fn(i, qkv)
         else:

@@ -261,6 +261,7 @@ class CausalLM(nn.Module):
             self.register_parameter(name.replace(".", "_"), prm)
         self.gradient_checkpointing = False
         self._rope_table: Optional[torch.Tensor] = None
+        self._rope_tables_before: List[torch.Tensor] = []
         if seed is not None:
             self.reset_parameters(seed)
 
@@ -298,23 +299,31 @@ class CausalLM(nn.Module):
             o, n = self.offsets[name]
             self._p[name].main_grad = flat_grad[o : o + n].view(shape)
 
-    def rope_table(self, device) -> torch.Tensor:
-        if self._rope_table is None or self._rope_table.device != torch.device(device):
+    def rope_table(self, device, positions: int = 0) -> torch.Tensor:
+        """cos | sin rows of the model's context, stretched where positions are scaled, and of at least ``positions``."""
+        t, device = self._rope_table, torch.device(device)
+        if t is None or t.device != device or t.shape[0] < positions:
             a = self.args
-            n = a.max_position_embeddings
-            if a.rope_scaling and "original_max_position_embeddings" in a.rope_scaling:  # the stretched context
-                n = max(n, int(a.rope_scaling["original_max_position_embeddings"] * float(a.rope_scaling["factor"])))
+            n = max(a.max_position_embeddings, positions)
+            if a.rope_scaling:
+                context = a.rope_scaling.get("original_max_position_embeddings", a.max_position_embeddings)
+                n = max(n, int(context * float(a.rope_scaling.get("factor", 1.0))))
+            if t is not None and t.device == device:
+                n = max(n, 2 * t.shape[0])  # seldom: captured graphs go on reading the tables before it
+                self._rope_tables_before.append(t)
             self._rope_table = ew.build_rope_table(n, a.rotary_dim, a.rope_theta, device, scaling=a.rope_scaling)
         return self._rope_table
 
     # ------------------------------------------------------------------ forward
-    def _rotate(self, i: int, qkv: torch.Tensor, pos: torch.Tensor, kv_sink=None, heads: Optional[Tuple[int, int]] = None):
+    def _rotate(self, i: int, qkv: torch.Tensor, pos: torch.Tensor, kv_sink=None, heads: Optional[Tuple[int, int]] = None,
+                max_seqlen: int = 0):
         """Fused projection rows -> normed (where the model has per-head norms) and rotated heads, handed to ``kv_sink``.
-        ``heads``: query and key heads of the rows where they are not all of the model's.  A sink with a ``paged(layer)``
+        ``heads``: query and key heads of the rows where they are not all of the model's.  ``max_seqlen``: positions lie below
+        it; a sequence beyond the model's context gets a longer table.  A sink with a ``paged(layer)``
         method (key cache, value cache, slots) gets its cache rows from the same launch; no gradients then."""
         a = self.args
         nq, nkv = heads or (a.num_heads, a.num_kv_heads)
-        table = self.rope_table(qkv.device)
+        table = self.rope_table(qkv.device, max_seqlen)
         if a.rotates_in_pass:
             pos = pos.to(torch.int32)
             qn, kn = (self.p(f"layers.{i}.q_norm"), self.p(f"layers.{i}.k_norm")) if a.qk_norm else (None, None)
@@ -338,7 +347,7 @@ class CausalLM(nn.Module):
         pre = f"layers.{i}."
         x, h = ew.add_rmsnorm(x, delta, self.p(pre + "ln1"), a.rms_norm_eps)
         qkv = gemm.linear(h, self.p(pre + "wqkv"), self._p.get(pre + "bqkv"))
-        qkv = self._rotate(i, qkv, pos, kv_sink)
+        qkv = self._rotate(i, qkv, pos, kv_sink, max_seqlen=max_seqlen)
         if attn_fn is not None:  # the caller supplies attention (e.g. over cached key/value prefixes)
             att = attn_fn(i, qkv)
         else:

@@ -143,7 +143,7 @@ class LoRACausalLM(CausalLM):
         pre = f"layers.{i}."
         x, h = ew.add_rmsnorm(x, delta, self.p(pre + "ln1"), a.rms_norm_eps)
         qkv = self._lin(i, "qkv", h, self._p.get(pre + "bqkv"))
-        qkv = self._rotate(i, qkv, pos, kv_sink)
+        qkv = self._rotate(i, qkv, pos, kv_sink, max_seqlen=max_seqlen)
         if attn_fn is not None:
             att = attn_fn(i, qkv)
         else:

@@ -261,7 +261,7 @@ class TPCausalLM(CausalLM):
         pre = f"layers.{i}."
         x, h = ew.add_rmsnorm(x, delta, self.p(pre + "ln1"), a.rms_norm_eps)  # [T/tp, H]
         qkv = tpm.column_parallel_linear(h, self.p(pre + "wqkv"), self._p.get(pre + "bqkv"), tp)  # [T, local heads]
-        qkv = self._rotate(i, qkv, pos)
+        qkv = self._rotate(i, qkv, pos, max_seqlen=max_seqlen)
         att = attn_ops.attn_varlen(qkv, cu, a.num_heads, a.num_kv_heads, a.head_dim, max_seqlen=max_seqlen)
         o = tpm.row_parallel_linear(att, self.p(pre + "wo"), tp)  # [T/tp, H]
         x, h = ew.add_rmsnorm(x, o, self.p(pre + "ln2"), a.rms_norm_eps)
@@ -364,7 +364,7 @@ class UlyssesCausalLM(CausalLM):
         x, h = ew.add_rmsnorm(x, delta, self.p(pre + "ln1"), a.rms_norm_eps)
         qkv = ulysses.qkv_proj(h, self.p(pre + "wqkv"), self._p.get(pre + "bqkv"), [a.q_dim, a.kv_dim, a.kv_dim], sp)
         nq, nkv = a.num_heads // sp.size, a.num_kv_heads // sp.size
-        qkv = self._rotate(i, qkv, pos, heads=(nq, nkv))
+        qkv = self._rotate(i, qkv, pos, heads=(nq, nkv), max_seqlen=max_seqlen)
         att = attn_ops.attn_varlen(qkv, cu, nq, nkv, a.head_dim, max_seqlen=max_seqlen)
         o = ulysses.o_proj(att, self.p(pre + "wo"), sp)
         x, h = ew.add_rmsnorm(x, o, self.p(pre + "ln2"), a.rms_norm_eps)
@@ -424,7 +424,7 @@ class ContextParallelCausalLM(UlyssesCausalLM):
         row0, row1, first, cu_loc, max_loc, q_begin = self._cp_plan
         x, h = ew.add_rmsnorm(x, delta, self.p(pre + "ln1"), a.rms_norm_eps)
         qkv = gemm.linear(h, self.p(pre + "wqkv"), self._p.get(pre + "bqkv"))
-        qkv = self._rotate(i, qkv, pos[row0:row1])
+        qkv = self._rotate(i, qkv, pos[row0:row1], max_seqlen=max_seqlen)
         kv_all = _AllGatherRowsSumBwdFn.apply(qkv[:, a.q_dim:].contiguous(), cp.group)  # [T, 2 * kv_dim]
         lead = row0 - first
         q_rows = qkv[:, : a.q_dim]
